@@ -4,6 +4,7 @@ The public names follow the reference package (comp_inference/__init__.py:13-59)
 implementation is a C-ABI HIP library (libcomp_inference_hip.so) driven through ctypes.
 """
 from . import ccore
+from .attention_hip import PagedKVCache, paged_attention, paged_kv_append, paged_kv_read, rotary_table
 from .comp_inference import (
     compressed_nbytes,
     extract_exp_and_mantissa,

@@ -20,5 +20,7 @@ extern "C" int ci_check_device(void) {
         return ci::fail(CI_ERR_DEVICE, "device %d is %s; this library holds gfx950 code only", dev,
                         prop.gcnArchName);
     // per-device set-up that must not happen for the first time inside a graph capture
+    uint32_t *word = nullptr;
+    if (int rc = ci::device_status_word(&word)) return rc;
     return ci_fused_linear_noalloc_init();
 }

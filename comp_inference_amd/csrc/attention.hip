@@ -1,0 +1,921 @@
+// Attention over the paged key/value cache (layout and matrix operands: paged.h).
+//
+//   out[i, h] = sum_j w_j v[j, g],  w = softmax over the visible keys j of scale * q[i, h] . k[j, g],  g = h / group
+//   query i of a sequence stands at position p = length - new tokens + i; key j is visible when j <= p and
+//   (no window, or p - j < window, or j < sinks)
+//
+// One pass over the keys with a running maximum and sum per row (both, and the output, in 32 bits; weights are rounded to
+// bf16 for the matrix instruction, one rounding of 2^-9 each, while their sum takes them unrounded).  The query heads that
+// share a kv head are rows of one product: row r of a sequence's kv head is (token r / group, head r % group).
+//
+// S^T = K Q^T puts queries into columns, so a lane holds 16 scores of ONE row and maximum and sum are lane arithmetic plus
+// one exchange between lane halves, and P^T is the operand of O^T = V^T P^T as it stands.
+//
+// Two kernels:
+//   attend_split_kernel   for few rows (single tokens): bound by reading the cache.  A tile is up to 32 rows; the blocks of
+//                         keys of all (sequence, tile, head) items form one list that is cut into equal shares, one per
+//                         workgroup, wherever the cut falls, so a batch of very different lengths fills the chip evenly.
+//                         An item that was cut is joined by attend_join_kernel.
+//   attend_rows_kernel    for many rows (prompts): bound by the matrix and vector units.  Four wavefronts of 32 rows share
+//                         the keys and values of a step of 64 tokens through the LDS.
+#include "paged.h"
+
+namespace ci {
+
+struct AttendArgs {
+    KvView cache;
+    KvBatch batch;
+    const uint16_t *q;
+    uint16_t *out;
+    float *lse;  // or nullptr: ln of the sum of exp(scores), [row, head]
+    int64_t q_row, q_head, o_row, o_head, l_row;
+    uint32_t group;  // query heads of a kv head
+    float scale_log2;  // scale * log2(e): the kernel works on powers of two
+    int32_t window, sinks;  // window 0: none
+    float *work;            // partial sums of cut items
+    uint32_t whole;         // 1: every item in one workgroup (no shares)
+};
+
+constexpr float kNone = -__builtin_inff();
+constexpr uint32_t kUnit = 4;  // blocks of a unit of work: one per wavefront
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float other_half(float x) {  // the value of lane ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float lane_xor(float x, int d) {
+    return __int_as_float(__shfl(__float_as_int(x), (int)(threadIdx.x & 63) ^ d, 64));
+}
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Rows [r0, r1) of a sequence, and the blocks of keys some of them see: [0, s1) and [w0, w0 + nb - s1).
+struct Span {
+    int32_t p_lo, p_hi;  // positions of the first and last row
+    uint32_t s1, w0, nb;
+    __device__ __forceinline__ uint32_t block(uint32_t i) const { return i < s1 ? i : i - s1 + w0; }
+};
+
+__device__ __forceinline__ Span span_of(const AttendArgs &a, const SeqInfo &s, uint32_t r0, uint32_t r1) {
+    Span x;
+    x.p_lo = s.len - s.n + (int32_t)(r0 / a.group);
+    x.p_hi = s.len - s.n + (int32_t)((r1 - 1) / a.group);
+    const uint32_t end = x.p_hi < 0 ? 0 : (uint32_t)x.p_hi / kKvBlock + 1;
+    x.s1 = x.w0 = 0;
+    if (a.window) {
+        x.w0 = x.p_lo - a.window + 1 > 0 ? (uint32_t)(x.p_lo - a.window + 1) / kKvBlock : 0;
+        x.s1 = min(((uint32_t)a.sinks + kKvBlock - 1) / kKvBlock, end);
+        if (x.s1 >= x.w0) x.s1 = x.w0 = 0;
+    }
+    x.nb = x.s1 + end - x.w0;
+    return x;
+}
+
+// Whether every row of the span sees every key of the block that starts at kb.
+__device__ __forceinline__ bool all_visible(const AttendArgs &a, const Span &x, int32_t kb) {
+    return kb + 31 <= x.p_lo && (!a.window || kb + 31 < a.sinks || kb > x.p_hi - a.window);
+}
+// Bits a .. b - 1 of a word (any a, b).
+__device__ __forceinline__ uint32_t bits(int32_t a, int32_t b) {
+    const uint32_t below_b = b >= 32 ? 0xFFFFFFFFu : b <= 0 ? 0u : (1u << b) - 1;
+    const uint32_t below_a = a >= 32 ? 0xFFFFFFFFu : a <= 0 ? 0u : (1u << a) - 1;
+    return below_b & ~below_a;
+}
+// The keys of the block at kb (a bit each) that some row at positions p_lo .. p_hi sees.
+__device__ __forceinline__ uint32_t seen_keys(const AttendArgs &a, int32_t p_lo, int32_t p_hi, int32_t kb) {
+    if (!a.window) return bits(0, p_hi + 1 - kb);
+    return bits(p_lo - a.window + 1 - kb, p_hi + 1 - kb) | bits(0, min(a.sinks, p_hi + 1) - kb);
+}
+
+__device__ __forceinline__ uint32_t rows_of(const AttendArgs &a, const SeqInfo &s) { return (uint32_t)s.n * a.group; }
+
+// ---- matrix operands ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ f32x16_p mfma(u32x4 x, u32x4 y, f32x16_p c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_p, x), __builtin_bit_cast(bf16x8_p, y), c, 0, 0, 0);
+}
+// Eight codes as bf16 numbers 128 + code: 0x4300 is 128 with seven fraction bits, the last four of which are the code.
+__device__ __forceinline__ u32x4 codes_to_bf16(uint32_t w) {
+    u32x4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = (w >> (4 * j) & 0x000F000Fu) | 0x43004300u;
+    return r;
+}
+__device__ __forceinline__ f32x16_p splat16(float x) {
+    f32x16_p r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = x;
+    return r;
+}
+
+template <int D>
+struct Queries {
+    u32x4 f[D / 16];
+    float sum;  // of all D channels
+};
+
+// Column `row` (of the rows of one kv head) as operand of S^T; columns at or beyond `rows` are zero.
+template <int D>
+__device__ __forceinline__ Queries<D> load_queries(const AttendArgs &a, const SeqInfo &s, uint32_t head, uint32_t row, uint32_t rows) {
+    Queries<D> q;
+    const uint32_t h = (threadIdx.x >> 5) & 1;
+    const bool there = row < rows;
+    const uint32_t tok = there ? row / a.group : 0, g = there ? row % a.group : 0;
+    const uint16_t *src = a.q + (int64_t)(s.row + (int32_t)tok) * a.q_row + (int64_t)(head * a.group + g) * a.q_head;
+    q.sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        q.f[i] = u32x4{0, 0, 0, 0};
+        if (there) q.f[i] = *reinterpret_cast<const u32x4 *>(src + 16 * i + 8 * h);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) q.sum += bf16_lo(q.f[i][w]) + bf16_hi(q.f[i][w]);
+    }
+    q.sum += other_half(q.sum);
+    return q;
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+// RP columns of the 32 are rows; the columns c, c + RP, c + 2 RP .. hold the same row.  Every one of them gets all 32 scores
+// of a block in the product, and works on 32 / RP of them only: column c + j RP takes elements [j NV, (j + 1) NV) of its
+// lane and puts zeros for the others into P^T, so O^T's columns are sums over disjoint sets of keys, each with a running
+// maximum of its own, joined once per item.  With four rows (a token of a model with four query heads per kv head) a lane
+// does the exponential of 2 scores per block instead of 16.
+template <int RP>
+struct Cols {
+    static constexpr int NJ = 32 / RP, NV = 16 / NJ;
+    uint32_t j;     // share of the lane's column
+    uint32_t key0;  // first key of its share: key of value i is key0 + (i & 3) + 8 (i >> 2)
+    __device__ __forceinline__ Cols() {
+        const uint32_t lane = threadIdx.x & 63;
+        j = (lane & 31) / RP;
+        key0 = ((j * NV) & 3) + 8 * ((j * NV) >> 2) + 4 * (lane >> 5);
+    }
+    __device__ __forceinline__ void take(const f32x16_p &s, float (&x)[NV]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] = s[i];
+#pragma unroll
+            for (int k = 1; k < NJ; ++k) x[i] = j == (uint32_t)k ? s[k * NV + i] : x[i];
+        }
+    }
+    // P^T operands of the two halves of a block from the lane's own weights
+    __device__ __forceinline__ void give(const uint32_t (&pk)[NV / 2], u32x4 (&f)[2]) const {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) f[w / 4][w % 4] = (NJ == 1 || j == (uint32_t)(w / (NV / 2))) ? pk[w % (NV / 2)] : 0u;
+    }
+    // bf16 pairs (step, low) of the lane's keys
+    __device__ __forceinline__ void pairs(const uint32_t *p, uint32_t (&x)[NV]) const {
+#pragma unroll
+        for (int i = 0; i < NV; i += 4) {
+            if (NV == 2) {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(p + key0);
+                x[0] = w[0], x[1] = w[1];
+            } else {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(p + key0 + 8 * (i >> 2));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[(i + k) % NV] = w[k];
+            }
+        }
+    }
+};
+
+// The running state of a lane's column: maximum (in powers of two, of the scaled scores), sum, output.
+template <int D>
+struct Running {
+    f32x16_p o[D / 32];
+    float m, l, off;  // off: what the 128 + code form of 4-bit values adds, to be taken out
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] = splat16(0.0f);
+        m = kNone;
+        l = off = 0.0f;
+    }
+    // Raises the maximum where a block exceeds it by more than 2^8 (weights stay below 2^8 otherwise, which costs bf16 and
+    // 32-bit sums no accuracy); what has been summed is scaled down only then.
+    __device__ __forceinline__ void raise(float block_max) {
+        if (__builtin_amdgcn_ballot_w64(block_max > m + 8.0f)) {
+            const float to = fmaxf(m, block_max), f = m == kNone ? 0.0f : exp2_fast(m - to);
+            m = to;
+            l *= f;
+            off *= f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[i][k] *= f;
+        }
+    }
+    __device__ __forceinline__ float base() const { return m == kNone ? 0.0f : m; }
+};
+
+// A value operand (s, h) without the keys that no row sees (what lies there need not be a number); `seen` has the lane's
+// key 0 of the operand's half, 4 h, as bit 0.
+__device__ __forceinline__ u32x4 keep_seen(u32x4 v, uint32_t seen, uint32_t s) {
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+        const uint32_t two = seen >> value_token(s, 0, 2 * w);
+        v[w] &= ((two & 1) ? 0x0000FFFFu : 0u) | ((two & 2) ? 0xFFFF0000u : 0u);
+    }
+    return v;
+}
+
+template <int KIND, int D>
+struct BlockData {  // keys and values of one block, as they lie in the cache
+    static constexpr int N = KIND == CI_KV_BF16 ? D / 16 : D / 64;
+    u32x4 k[N], v[N];
+};
+
+struct Item {
+    uint32_t seq, tile, head;
+};
+
+// What the units of one (sequence, tile) are; every head of it has the same.
+template <int RP>
+__device__ __forceinline__ uint32_t units_of(const AttendArgs &a, const SeqInfo &s, uint32_t tile) {
+    const uint32_t r0 = tile * RP, r1 = min(r0 + RP, rows_of(a, s));
+    return max((span_of(a, s, r0, r1).nb + kUnit - 1) / kUnit, 1u);
+}
+template <int RP>
+__device__ __forceinline__ uint32_t tiles_of(const AttendArgs &a, const SeqInfo &s) { return (rows_of(a, s) + RP - 1) / RP; }
+
+// Units of a sequence over all its tiles and heads.
+template <int RP>
+__device__ __forceinline__ uint32_t weight_of(const AttendArgs &a, uint32_t i) {
+    bool bad;
+    const SeqInfo s = load_seq(a.batch, a.cache, i, bad);
+    uint32_t n = 0;
+    for (uint32_t t = 0; t < tiles_of<RP>(a, s); ++t) n += units_of<RP>(a, s, t);
+    return n * a.cache.kv_heads;
+}
+template <int RP>
+__device__ __forceinline__ uint32_t items_of(const AttendArgs &a, uint32_t i) {
+    bool bad;
+    return tiles_of<RP>(a, load_seq(a.batch, a.cache, i, bad)) * a.cache.kv_heads;
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
+// Item number `index` of the batch.
+template <int RP>
+__device__ __forceinline__ bool find_item(const AttendArgs &a, uint32_t index, uint32_t *word, Item &it) {
+    uint32_t begin;
+    if (!a.batch.start && a.group <= RP) {  // one tile per sequence
+        it.seq = index / a.cache.kv_heads;
+        begin = it.seq * a.cache.kv_heads;
+        if (it.seq >= a.batch.seqs) return false;
+    } else {
+        Found f;
+        if (!locate(a.batch.seqs, [&](uint32_t i) { return items_of<RP>(a, i); }, [&](uint32_t) { return index; }, word, f))
+            return false;
+        it.seq = f.seq;
+        begin = f.begin;
+    }
+    it.tile = (index - begin) / a.cache.kv_heads;
+    it.head = (index - begin) % a.cache.kv_heads;
+    return true;
+}
+
+// One workgroup's part of one item: units [u0, u1).  Joins its wavefronts and columns in the LDS, and writes the result:
+// the item's rows, or (part of an item) the partial sums of RP rows to `slot`.
+template <int KIND, int D, int RP>
+__device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it, const SeqInfo &s, uint32_t u0, uint32_t u1,
+                                             bool whole, float *slot, uint8_t *lds) {
+    constexpr int NV = Cols<RP>::NV, NJ = Cols<RP>::NJ;
+    constexpr uint32_t kStride = D + 4;  // floats of a column in the LDS (the four spread the columns over the banks)
+    typedef BlockData<KIND, D> Data;
+    const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const uint32_t r0 = it.tile * RP, rows = min((uint32_t)RP, rows_of(a, s) - r0);
+    const Span span = span_of(a, s, r0, r0 + rows);
+    const Cols<RP> cols;
+    const uint32_t row = col % RP;
+    const Queries<D> q = load_queries<D>(a, s, it.head, r0 + row, r0 + rows);
+    const int32_t pos = s.len - s.n + (int32_t)((r0 + row) / a.group);
+    Running<D> run;
+    run.clear();
+    const f32x16_p start = splat16(KIND == CI_KV_BF16 ? 0.0f : -128.0f * q.sum);
+    const uint32_t last = min(u1 * kUnit, span.nb);
+    bool lost = false;
+
+    auto fetch_k = [&](const uint8_t *b, Data &x) {
+#pragma unroll
+        for (int i = 0; i < Data::N; ++i) x.k[i] = reinterpret_cast<const u32x4 *>(b)[i * 64 + lane];
+    };
+    auto fetch_v = [&](const uint8_t *b, Data &x) {
+#pragma unroll
+        for (int i = 0; i < Data::N; ++i) x.v[i] = reinterpret_cast<const u32x4 *>(b + KvBlock<KIND, D>::kHalf)[i * 64 + lane];
+    };
+    // the block of a step; a page that is none of the cache's: some page, its keys unseen
+    auto place = [&](uint32_t i, bool &gone) -> const uint8_t * {
+        const uint32_t blk = span.block(i);
+        const uint32_t page = uniform(page_of(a.batch, a.cache, it.seq, blk));
+        gone = page == kNoPage;
+        return block_at<KIND, D>(a.cache, gone ? 0 : page, it.head, blk);
+    };
+
+    // keys are asked for one step ahead, values at the head of their step: a wavefront always has half a block on its way
+    Data x;
+    uint32_t i = u0 * kUnit + wave;
+    const uint8_t *b = nullptr;
+    bool gone_next = false;
+    if (i < last) {
+        b = place(i, gone_next);
+        fetch_k(b, x);
+    }
+    for (; i < last; i += kUnit) {
+        const int32_t kb = (int32_t)(span.block(i) * kKvBlock);
+        const bool gone = gone_next;
+        lost = lost || gone;
+        fetch_v(b, x);
+        const bool edge = gone || !all_visible(a, span, kb);
+        uint32_t sees = 0xFFFFFFFFu;  // the lane's keys that its row sees, key0 as bit 0
+        if (edge) sees = gone ? 0u : seen_keys(a, pos, pos, kb) >> cols.key0;
+        f32x16_p acc = start;
+        if (KIND == CI_KV_BF16) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) acc = mfma(x.k[k], q.f[k], acc);
+        } else {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) acc = mfma(codes_to_bf16(x.k[k / 4][k % 4]), q.f[k], acc);
+        }
+        uint32_t kp[NV], vp[NV];
+        if (KIND != CI_KV_BF16) {
+            const uint32_t *pairs = reinterpret_cast<const uint32_t *>(b + KvBlock<KIND, D>::kPairs);
+            cols.pairs(pairs, kp);
+            cols.pairs(pairs + kKvBlock, vp);
+        }
+        b = place(min(i + kUnit, last - 1), gone_next);
+        fetch_k(b, x);
+        float t[NV];
+        cols.take(acc, t);
+        float best = kNone;
+#pragma unroll
+        for (int e = 0; e < NV; ++e) {
+            if (KIND != CI_KV_BF16) t[e] = t[e] * bf16_lo(kp[e]) + q.sum * bf16_hi(kp[e]);
+            t[e] *= a.scale_log2;
+            if (edge) t[e] = sees >> ((e & 3) + 8 * (e >> 2)) & 1 ? t[e] : kNone;
+            best = fmaxf(best, t[e]);
+        }
+        run.raise(max_halves(best));
+        const float base = run.base();
+        uint32_t pk[NV / 2];
+#pragma unroll
+        for (int e = 0; e < NV; e += 2) {
+            float p0 = exp2_fast(t[e] - base), p1 = exp2_fast(t[e + 1] - base);
+            run.l += p0 + p1;
+            if (KIND == CI_KV_BF16) {
+                pk[e / 2] = bf16_pair(p0, p1);
+            } else {
+                // o = sum p (low + step code): the step goes into the weight, the low and the 128 of the code into `off`;
+                // a key that is not seen weighs nothing, whatever its step and low are
+                const float s0 = p0 * bf16_lo(vp[e]), s1 = p1 * bf16_lo(vp[e + 1]);
+                float l0 = p0 * bf16_hi(vp[e]), l1 = p1 * bf16_hi(vp[e + 1]);
+                pk[e / 2] = bf16_pair(s0, s1);
+                if (edge) {
+                    const bool z0 = t[e] == kNone, z1 = t[e + 1] == kNone;
+                    l0 = z0 ? 0.0f : l0;
+                    l1 = z1 ? 0.0f : l1;
+                    pk[e / 2] &= (z0 ? 0u : 0xFFFFu) | (z1 ? 0u : 0xFFFF0000u);
+                }
+                run.off += l0 + l1 - 128.0f * (bf16_lo(pk[e / 2]) + bf16_hi(pk[e / 2]));
+            }
+        }
+        u32x4 f[2];
+        cols.give(pk, f);
+        if (KIND == CI_KV_BF16 && edge) {
+            const uint32_t seen = gone ? 0u : seen_keys(a, span.p_lo, span.p_hi, kb) >> (4 * h);
+#pragma unroll
+            for (int k = 0; k < Data::N; ++k) x.v[k] = keep_seen(x.v[k], seen, (uint32_t)k / (D / 32));
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db) {
+                const int k = s2 * (D / 32) + db;
+                run.o[db] = mfma(KIND == CI_KV_BF16 ? x.v[k % Data::N] : codes_to_bf16(x.v[k / 4][k % 4]), f[s2], run.o[db]);
+            }
+    }
+    if (lost && lane == 0) report_bad_index(a.batch);
+
+    // ---- join: the columns of a wavefront that hold the same row (c, c + RP, ..), then the four wavefronts
+    float *o_lds = reinterpret_cast<float *>(lds);                      // [4][32][kStride]
+    float *m_lds = o_lds + 4 * 32 * kStride, *l_lds = m_lds + 4 * RP;  // [4][RP] each
+    run.l += other_half(run.l);
+    run.off += other_half(run.off);
+    float m = run.m;
+#pragma unroll
+    for (int d = RP; d < 32; d *= 2) m = fmaxf(m, lane_xor(m, d));
+    const float f = run.m == kNone ? 0.0f : exp2_fast(run.m - m);
+    float l = run.l * f;  // (a NaN stays one: 0 x NaN)
+#pragma unroll
+    for (int d = RP; d < 32; d *= 2) l += lane_xor(l, d);
+    __syncthreads();  // (the LDS is free of the piece before)
+    if (lane < RP) {
+        m_lds[wave * RP + lane] = m;
+        l_lds[wave * RP + lane] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f32x4_p w;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = f * (run.o[db][4 * k + c] + (KIND == CI_KV_BF16 ? 0.0f : run.off));
+            *reinterpret_cast<f32x4_p *>(o_lds + (wave * 32 + col) * kStride + 32 * db + 8 * k + 4 * h) = w;
+        }
+    __syncthreads();
+    for (uint32_t o = threadIdx.x; o < rows * (D / 4); o += 256) {
+        const uint32_t rr = o / (D / 4), d = o % (D / 4) * 4;
+        const float top = fmaxf(fmaxf(m_lds[rr], m_lds[RP + rr]), fmaxf(m_lds[2 * RP + rr], m_lds[3 * RP + rr]));
+        f32x4_p acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+#pragma unroll 1
+        for (uint32_t w = 0; w < 4; ++w) {
+            const float mw = m_lds[w * RP + rr], fw = mw == kNone ? 0.0f : exp2_fast(mw - top);
+            l += fw * l_lds[w * RP + rr];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const f32x4_p y = *reinterpret_cast<const f32x4_p *>(o_lds + (w * 32 + j * RP + rr) * kStride + d);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[c] += fw * y[c];
+            }
+        }
+        if (whole) {
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing: zeros)
+            const uint32_t tok = (r0 + rr) / a.group, g = (r0 + rr) % a.group;
+            u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+            *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row +
+                                       (int64_t)(it.head * a.group + g) * a.o_head + d) = w;
+            if (a.lse && d == 0)
+                a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + it.head * a.group + g] =
+                    top == kNone ? kNone : (top + log2f(l)) * 0.6931471805599453f;
+        } else {
+            *reinterpret_cast<f32x4_p *>(slot + rr * D + d) = acc;
+            if (d == 0) {
+                slot[RP * D + rr] = top;
+                slot[RP * D + RP + rr] = l;
+            }
+        }
+    }
+}
+
+template <int D, int RP>
+constexpr uint32_t slot_floats() { return RP * (D + 2); }
+constexpr uint32_t split_lds(int D) { return (4 * 32 * (D + 4) + 2 * 4 * 32) * 4; }
+
+// Units of all items in the order (sequence, tile, head), cut evenly.
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t workers) { return max((total + workers - 1) / workers, 1u); }
+
+template <int KIND, int D, int RP>
+__global__ __launch_bounds__(256, 2) void attend_split_kernel(AttendArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t *word = reinterpret_cast<uint32_t *>(lds);
+    Item it;
+    bool bad;
+    // the share of this workgroup, and the item it begins in: one item, or units [at, end) of the batch's
+    uint32_t at = 0, end = 0, u0 = 0, units = 0;
+    SeqInfo s;
+    if (a.whole) {
+        if (!find_item<RP>(a, blockIdx.x, word, it)) return;
+        s = load_seq(a.batch, a.cache, it.seq, bad);
+        end = units = units_of<RP>(a, s, it.tile);
+    } else {
+        Found f;
+        if (!locate(a.batch.seqs, [&](uint32_t i) { return weight_of<RP>(a, i); },
+                    [&](uint32_t total) { return blockIdx.x * share_of(total, gridDim.x); }, word, f))
+            return;
+        it.seq = f.seq;
+        at = f.target;
+        end = min(at + share_of(f.total, gridDim.x), f.total);
+        s = load_seq(a.batch, a.cache, it.seq, bad);
+        uint32_t inside = at - f.begin;  // unit inside the sequence
+        for (it.tile = 0;; ++it.tile) {
+            units = units_of<RP>(a, s, it.tile);
+            if (inside < units * a.cache.kv_heads) break;
+            inside -= units * a.cache.kv_heads;
+        }
+        it.head = inside / units;
+        u0 = inside % units;
+    }
+    for (;;) {
+        if (bad && threadIdx.x == 0) report_bad_index(a.batch);
+        const uint32_t u1 = min(units, u0 + end - at);
+        // an item that goes on from the workgroup before leaves its sums in slot 0, one that goes on in the next in slot 1
+        float *slot = a.work + (uint64_t)(blockIdx.x * 2 + (u0 == 0 ? 1 : 0)) * slot_floats<D, RP>();
+        attend_piece<KIND, D, RP>(a, it, s, u0, u1, u0 == 0 && u1 == units, slot, lds);
+        at += u1 - u0;
+        if (at >= end) break;
+        u0 = 0;
+        if (++it.head < a.cache.kv_heads) continue;
+        it.head = 0;
+        if (++it.tile >= tiles_of<RP>(a, s)) {
+            it.tile = 0;
+            do {
+                if (++it.seq >= a.batch.seqs) return;
+                s = load_seq(a.batch, a.cache, it.seq, bad);
+            } while (s.n == 0);
+        }
+        units = units_of<RP>(a, s, it.tile);
+    }
+}
+
+// One row of one item that was cut: the sum of its parts, which 256 / (D / 4) groups of threads take in turn.
+template <int D, int RP>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t workers) {
+    constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
+    __shared__ uint32_t word[8];
+    __shared__ float part[256 * 4];
+    __shared__ float part_l[16];
+    Item it;
+    if (!find_item<RP>(a, blockIdx.x, word, it)) return;
+    bool bad;
+    const SeqInfo s = load_seq(a.batch, a.cache, it.seq, bad);
+    const uint32_t r0 = it.tile * RP, rows = min((uint32_t)RP, rows_of(a, s) - r0), row = blockIdx.y;
+    if (row >= rows) return;
+    // where the item's units begin
+    uint32_t total, before = 0;
+    {
+        const uint32_t per = (a.batch.seqs + 255) / 256, first = min(threadIdx.x * per, a.batch.seqs);
+        const uint32_t end = min(first + per, a.batch.seqs);
+        uint32_t mine = 0;
+        for (uint32_t i = first; i < end; ++i) mine += weight_of<RP>(a, i);
+        before = scan256(mine, word, total);
+        if (it.seq >= first && it.seq < end) {
+            for (uint32_t i = first; i < it.seq; ++i) before += weight_of<RP>(a, i);
+            word[6] = before;
+        }
+        __syncthreads();
+        before = uniform(word[6]);
+        total = uniform(total);
+    }
+    for (uint32_t t = 0; t < it.tile; ++t) before += units_of<RP>(a, s, t) * a.cache.kv_heads;
+    const uint32_t units = units_of<RP>(a, s, it.tile);
+    before += it.head * units;
+    const uint32_t share = share_of(total, workers), w0 = before / share, w1 = (before + units - 1) / share;
+    if (w0 == w1) return;  // (written whole)
+    const uint32_t g = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    float m = kNone;
+    for (uint32_t w = w0; w <= w1; ++w)
+        m = fmaxf(m, a.work[(uint64_t)(w * 2 + (w == w0 ? 1 : 0)) * slot_floats<D, RP>() + RP * D + row]);
+    f32x4_p acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (uint32_t w = w0 + g; w <= w1; w += kGroups) {
+        const float *slot = a.work + (uint64_t)(w * 2 + (w == w0 ? 1 : 0)) * slot_floats<D, RP>();
+        const float mw = slot[RP * D + row], f = mw == kNone ? 0.0f : exp2_fast(mw - m);
+        const f32x4_p y = *reinterpret_cast<const f32x4_p *>(slot + row * D + d);
+        l += f * slot[RP * D + RP + row];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
+    }
+    *reinterpret_cast<f32x4_p *>(part + threadIdx.x * 4) = acc;
+    if (d == 0) part_l[g] = l;
+    __syncthreads();
+    if (threadIdx.x >= kLanes) return;
+    l = 0.0f;
+    acc = f32x4_p{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t k = 0; k < kGroups; ++k) {
+        l += part_l[k];
+        const f32x4_p y = *reinterpret_cast<const f32x4_p *>(part + (k * kLanes + threadIdx.x) * 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += y[c];
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const uint32_t tok = (r0 + row) / a.group, gh = it.head * a.group + (r0 + row) % a.group;
+    u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+    *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
+    if (a.lse && d == 0)
+        a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// ---- many rows ------------------------------------------------------------------------------------------------------
+constexpr uint32_t kTileRows = 128;  // four wavefronts of 32
+constexpr uint32_t rows_lds(int D) { return 2 * 2 * 128 * D; }  // two buffers of two blocks, keys and values in bf16
+
+// What a thread carries of the next step from memory to the LDS.
+template <int KIND, int D>
+struct Stage;
+
+// bf16: blocks are copied as they lie.
+template <int D>
+struct Stage<CI_KV_BF16, D> {
+    static constexpr int N = D / 16;  // 16-byte pieces per thread: 2 blocks x 128 D bytes / 4096
+    u32x4 x[N];
+    __device__ __forceinline__ void fetch(const uint8_t *b0, const uint8_t *b1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x[i] = reinterpret_cast<const u32x4 *>(i < N / 2 ? b0 : b1)[(i % (N / 2)) * 256 + threadIdx.x];
+    }
+    __device__ __forceinline__ void store(uint8_t *lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) reinterpret_cast<u32x4 *>(lds)[i * 256 + threadIdx.x] = x[i];
+    }
+};
+
+// 4 bits: the codes become the values they stand for, rounded to bf16 (what a bf16 cache would hold of them), once for the
+// four wavefronts that use them.  A wavefront takes whole 1 KB pieces: for heads of 128 keys (wavefronts 0, 1) or values
+// (2, 3) of both blocks, for heads of 64 keys or values of one block.
+template <int D>
+struct Stage<CI_KV_INT4, D> {
+    static constexpr int N = D / 64, U = N;  // pieces of the keys of a block; pieces per wavefront: 2 * 2 * N / 4
+    u32x4 x[U];
+    uint32_t pair[16];
+    static __device__ __forceinline__ uint32_t unit(int u) { return uniform(threadIdx.x >> 6) + 4 * u; }
+    __device__ __forceinline__ void fetch(const uint8_t *b0, const uint8_t *b1) {
+        const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
+            const uint8_t *b = blk ? b1 : b0;
+            x[u] = reinterpret_cast<const u32x4 *>(b + values * KvBlock<CI_KV_INT4, D>::kHalf)[i * 64 + lane];
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(b + KvBlock<CI_KV_INT4, D>::kPairs);
+            const uint32_t key = p[lane & 31];
+#pragma unroll
+            for (int c = 0; c < 16 / U; c += 4) {  // tokens 16 s + 8 a + 4 h + b, s = i for heads of 128
+                const uint32_t s = U == 2 ? i : c / 8;
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(p + kKvBlock + 16 * s + 8 * (c / 4 % 2) + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pair[u * 8 + c + e] = w[e];
+            }
+            if (!values) pair[u * 8] = key;
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t *lds) const {
+        const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
+            u32x4 *dst = reinterpret_cast<u32x4 *>(lds + blk * 128 * D + values * 64 * D);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const u32x4 n = codes_to_bf16(x[u][c]);  // 128 + code
+                u32x4 y;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int at = u * 8 + (U == 2 ? 0 : c / 2 * 8) + 2 * w;
+                    const uint32_t key = pair[u * 8], v0 = pair[at], v1 = pair[at + 1];
+                    const uint32_t p0 = values ? v0 : key, p1 = values ? v1 : key;
+                    y[w] = bf16_pair(fmaf(bf16_lo(p0), bf16_lo(n[w]) - 128.0f, bf16_hi(p0)),
+                                     fmaf(bf16_lo(p1), bf16_hi(n[w]) - 128.0f, bf16_hi(p1)));
+                }
+                dst[(i * 4 + c) * 64 + lane] = y;
+            }
+        }
+    }
+};
+
+template <int KIND, int D>
+__global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t *word = reinterpret_cast<uint32_t *>(lds);
+    // Workgroups go to the eight XCDs in turn, and each has an L2 of its own: an XCD takes a contiguous run of the items in
+    // the order (sequence, head, tile), so that the tiles of a head read its keys and values through one L2.
+    Found f;
+    const auto items = [&](uint32_t i) {
+        bool x;
+        return (rows_of(a, load_seq(a.batch, a.cache, i, x)) + kTileRows - 1) / kTileRows * a.cache.kv_heads;
+    };
+    const auto mine = [&](uint32_t total) {
+        const uint32_t run = (total + 7) / 8, k = blockIdx.x >> 3;
+        return k < run ? (blockIdx.x & 7) * run + k : 0xFFFFFFFFu;
+    };
+    if (!locate(a.batch.seqs, items, mine, word, f)) return;
+    bool bad;
+    const SeqInfo s = load_seq(a.batch, a.cache, f.seq, bad);
+    if (bad && threadIdx.x == 0) report_bad_index(a.batch);
+    const uint32_t all_rows = rows_of(a, s), tiles = (all_rows + kTileRows - 1) / kTileRows;
+    const uint32_t head = (f.target - f.begin) / tiles, tile = tiles - 1 - (f.target - f.begin) % tiles;  // (longest first)
+    const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+    const uint32_t t0 = tile * kTileRows, t1 = min(t0 + kTileRows, all_rows);
+    const Span span = span_of(a, s, t0, t1);
+    const uint32_t r0 = t0 + wave * 32, r1 = min(r0 + 32, t1);
+    const bool any = r0 < r1;
+    Span own = any ? span_of(a, s, r0, r1) : span;
+    const Queries<D> q = load_queries<D>(a, s, head, r0 + col, t1);
+    const int32_t pos = s.len - s.n + (int32_t)((r0 + col) / a.group);
+    Running<D> run;
+    run.clear();
+
+    const auto place = [&](uint32_t i, bool &gone) -> const uint8_t * {
+        const uint32_t blk = span.block(min(i, span.nb - 1));
+        const uint32_t page = page_of(a.batch, a.cache, f.seq, blk);
+        gone = page == kNoPage;
+        return block_at<KIND, D>(a.cache, gone ? 0 : page, head, blk);
+    };
+    Stage<KIND, D> stage;
+    bool gone[2] = {false, false}, lost = false;
+    const uint32_t steps = (span.nb + 1) / 2;
+    if (steps) {
+        const uint8_t *b0 = place(0, gone[0]), *b1 = place(1, gone[1]);
+        stage.fetch(b0, b1);
+    }
+    for (uint32_t st = 0; st < steps; ++st) {
+        uint8_t *buf = lds + (st & 1) * (256 * D);
+        stage.store(buf);
+        const bool g0 = gone[0], g1 = gone[1] || 2 * st + 1 >= span.nb;
+        lost = lost || g0 || gone[1];
+        __syncthreads();
+        if (st + 1 < steps) {
+            const uint8_t *b0 = place(2 * st + 2, gone[0]), *b1 = place(2 * st + 3, gone[1]);
+            stage.fetch(b0, b1);
+        }
+        const int32_t kb0 = (int32_t)(span.block(2 * st) * kKvBlock);
+        const int32_t kb1 = (int32_t)(span.block(min(2 * st + 1, span.nb - 1)) * kKvBlock);
+        // a wavefront none of whose rows sees a key of either block has nothing to do in this step
+        const int32_t lo = a.window ? own.p_lo - a.window + 1 : 0;
+        const auto seen = [&](int32_t kb) { return kb <= own.p_hi && (kb + 31 >= lo || kb < a.sinks); };
+        if (!any || !((seen(kb0) && !g0) || (seen(kb1) && !g1))) continue;
+
+        const u32x4 *kv = reinterpret_cast<const u32x4 *>(buf);
+        constexpr int kBlk = 8 * D;  // 16-byte pieces of a block: keys, then values
+        f32x16_p acc0 = splat16(0.0f), acc1 = acc0;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            acc0 = mfma(kv[k * 64 + lane], q.f[k], acc0);
+            acc1 = mfma(kv[kBlk + k * 64 + lane], q.f[k], acc1);
+        }
+        const bool edge = g0 || g1 || !all_visible(a, own, kb0) || !all_visible(a, own, kb1);
+        uint32_t seen0 = 0, seen1 = 0;  // of the wavefront's rows, from key 4 h on
+        if (edge) {
+            const uint32_t s0 = g0 ? 0u : seen_keys(a, pos, pos, kb0) >> (4 * h), s1 = g1 ? 0u : seen_keys(a, pos, pos, kb1) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                acc0[e] = s0 >> ((e & 3) + 8 * (e >> 2)) & 1 ? acc0[e] : kNone;
+                acc1[e] = s1 >> ((e & 3) + 8 * (e >> 2)) & 1 ? acc1[e] : kNone;
+            }
+            seen0 = g0 ? 0u : seen_keys(a, own.p_lo, own.p_hi, kb0) >> (4 * h);
+            seen1 = g1 ? 0u : seen_keys(a, own.p_lo, own.p_hi, kb1) >> (4 * h);
+        }
+        float best = kNone;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) best = fmaxf(best, fmaxf(acc0[e], acc1[e]));
+        run.raise(max_halves(best) * a.scale_log2);
+        const float base = run.base();
+        u32x4 p[4];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            const float x0 = exp2_fast(acc0[e] * a.scale_log2 - base), x1 = exp2_fast(acc0[e + 1] * a.scale_log2 - base);
+            const float y0 = exp2_fast(acc1[e] * a.scale_log2 - base), y1 = exp2_fast(acc1[e + 1] * a.scale_log2 - base);
+            run.l += (x0 + x1) + (y0 + y1);
+            p[e / 8][e / 2 % 4] = bf16_pair(x0, x1);
+            p[2 + e / 8][e / 2 % 4] = bf16_pair(y0, y1);
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 4; ++s2)
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db) {
+                u32x4 v = kv[(s2 / 2) * kBlk + 4 * D + ((s2 % 2) * (D / 32) + db) * 64 + lane];
+                if (edge) v = keep_seen(v, s2 < 2 ? seen0 : seen1, s2 % 2);
+                run.o[db] = mfma(v, p[s2], run.o[db]);
+            }
+    }
+    if (lost && threadIdx.x == 0) report_bad_index(a.batch);
+    const float l = run.l + other_half(run.l), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    if (r0 + col >= t1) return;
+    const uint32_t tok = (r0 + col) / a.group, gh = head * a.group + (r0 + col) % a.group;
+    uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            u32x2 w = {bf16_pair(run.o[db][4 * k] * inv, run.o[db][4 * k + 1] * inv),
+                       bf16_pair(run.o[db][4 * k + 2] * inv, run.o[db][4 * k + 3] * inv)};
+            *reinterpret_cast<u32x2 *>(dst + 32 * db + 8 * k + 4 * h) = w;
+        }
+    if (a.lse && h == 0)
+        a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = run.m == kNone ? kNone : (run.m + log2f(l)) * 0.6931471805599453f;
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+struct AttendPlan {
+    bool many;         // attend_rows_kernel
+    bool whole;        // split kernel, one workgroup per item
+    uint32_t rp, grid, items, workers;
+    size_t work_bytes;
+};
+
+// `longest`, `new_longest`: the caller's bounds on the lengths.  They choose kernels; the results do not rest on them.
+static int plan_attend(const KvView &v, const KvBatch &b, uint32_t head_dim, uint32_t group, int32_t window, int32_t sinks,
+                       uint32_t new_longest, uint32_t longest, AttendPlan *p) {
+    uint32_t cus = 1;
+    if (int rc = cu_count(&cus)) return rc;
+    const uint64_t rows = (uint64_t)b.tokens * group;
+    const uint64_t per_seq = (uint64_t)(b.start ? new_longest : 1) * group;
+    p->many = per_seq >= 64 && rows * v.kv_heads / kTileRows >= cus / 2;
+    p->whole = false;
+    p->work_bytes = 0;
+    p->rp = per_seq <= 4 ? 4 : per_seq <= 8 ? 8 : per_seq <= 16 ? 16 : 32;
+    const uint64_t tiles = b.start ? rows / (p->many ? kTileRows : p->rp) + b.seqs : (uint64_t)b.seqs * ceil_div(group, p->rp);
+    const uint64_t items = tiles * v.kv_heads;
+    if (items > 0x7FFFFF00ull) return fail(CI_ERR_ARG, "ci_paged_attention: too many rows for one call");
+    p->items = (uint32_t)items;
+    if (p->many) {
+        p->grid = (p->items + 7) / 8 * 8;
+        return CI_OK;
+    }
+    uint64_t keys = longest;
+    if (window && (uint64_t)window + sinks + 64 < keys) keys = (uint64_t)window + sinks + 64;
+    p->whole = keys <= 4 * kUnit * kKvBlock;
+    p->workers = 2 * cus;
+    p->grid = p->whole ? p->items : p->workers;
+    if (!p->whole) p->work_bytes = (size_t)p->workers * 2 * p->rp * (head_dim + 2) * sizeof(float);
+    return CI_OK;
+}
+
+template <int KIND, int D, int RP>
+static int launch_split(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+    CI_ALLOW_FULL_LDS((attend_split_kernel<KIND, D, RP>));
+    CI_KV_LAUNCH((attend_split_kernel<KIND, D, RP>), dim3(p.grid), dim3(256), split_lds(D), s, a);
+    CI_LAUNCH_CHECK("attend_split_kernel");
+    if (!p.whole) {
+        CI_KV_LAUNCH((attend_join_kernel<D, RP>), dim3(p.items, RP), dim3(256), 0, s, a, p.workers);
+        CI_LAUNCH_CHECK("attend_join_kernel");
+    }
+    return CI_OK;
+}
+
+template <int KIND, int D>
+static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+    if (p.many) {
+        CI_ALLOW_FULL_LDS((attend_rows_kernel<KIND, D>));
+        CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(256), rows_lds(D), s, a);
+        CI_LAUNCH_CHECK("attend_rows_kernel");
+        return CI_OK;
+    }
+    switch (p.rp) {
+        case 4: return launch_split<KIND, D, 4>(a, p, s);
+        case 8: return launch_split<KIND, D, 8>(a, p, s);
+        case 16: return launch_split<KIND, D, 16>(a, p, s);
+        default: return launch_split<KIND, D, 32>(a, p, s);
+    }
+}
+
+static int check_attend(const char *who, const ci_kv_cache *cache, const ci_kv_batch *batch, uint32_t q_heads, int32_t window,
+                        int32_t sinks, KvView *v, KvBatch *b) {
+    if (int rc = check_kv_cache(who, cache, v)) return rc;
+    if (int rc = check_kv_batch(who, batch, *v, b)) return rc;
+    if (q_heads == 0 || q_heads % v->kv_heads || q_heads > 65536)
+        return fail(CI_ERR_ARG, "%s: q_heads must be a multiple of kv_heads", who);
+    if (window < 0 || sinks < 0) return fail(CI_ERR_ARG, "%s: window and sinks must not be negative", who);
+    if ((uint64_t)b->tokens * (q_heads / v->kv_heads) > 0x7FFFFF00ull)
+        return fail(CI_ERR_ARG, "%s: too many rows for one call", who);
+    return CI_OK;
+}
+
+}  // namespace ci
+
+using namespace ci;
+
+extern "C" size_t ci_paged_attention_workspace_bytes(const ci_kv_cache *cache, const ci_kv_batch *batch, uint32_t q_heads,
+                                                     int32_t window, int32_t sinks, uint32_t max_query_len,
+                                                     uint32_t max_seq_len) {
+    KvView v;
+    KvBatch b;
+    AttendPlan p;
+    if (check_attend("ci_paged_attention_workspace_bytes", cache, batch, q_heads, window, sinks, &v, &b)) return 0;
+    if (b.seqs == 0 || b.tokens == 0) return 0;
+    if (plan_attend(v, b, cache->head_dim, q_heads / v.kv_heads, window, sinks, max_query_len ? max_query_len : b.tokens,
+                    max_seq_len ? max_seq_len : b.table_width << (v.page_shift + 5), &p))
+        return 0;
+    return p.work_bytes;
+}
+
+extern "C" int ci_paged_attention(const ci_kv_cache *cache, const ci_kv_batch *batch, const ci_rows *q, const ci_rows *out,
+                                  float *d_lse, int64_t lse_stride, uint32_t q_heads, float scale, int32_t window,
+                                  int32_t sinks, uint32_t max_query_len, uint32_t max_seq_len, void *d_workspace,
+                                  size_t workspace_bytes, ci_stream_t stream) {
+    static const char *who = "ci_paged_attention";
+    AttendArgs a{};
+    if (int rc = check_attend(who, cache, batch, q_heads, window, sinks, &a.cache, &a.batch)) return rc;
+    if (!q || !out) return fail(CI_ERR_ARG, "%s: null q or out", who);
+    if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(CI_ERR_ARG, "%s: scale must be positive and finite", who);
+    if (a.batch.seqs == 0 || a.batch.tokens == 0) return CI_OK;
+    for (const ci_rows *r : {q, out}) {
+        if (!r->d_data || !aligned(r->d_data, 16) || r->row_stride % 8 || r->head_stride % 8 || r->row_stride < 0 || r->head_stride < 0)
+            return fail(CI_ERR_ARG, "%s: %s must be a 16-byte aligned device pointer with strides that are non-negative multiples of 8",
+                        who, r == q ? "q" : "out");
+    }
+    a.q = static_cast<const uint16_t *>(q->d_data);
+    a.out = static_cast<uint16_t *>(out->d_data);
+    a.lse = d_lse;
+    a.l_row = lse_stride;
+    a.q_row = q->row_stride, a.q_head = q->head_stride, a.o_row = out->row_stride, a.o_head = out->head_stride;
+    a.group = q_heads / a.cache.kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.window = window < (1 << 30) ? window : 1 << 30;  // (no sequence is longer: sums of positions stay in 32 bits)
+    a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
+    AttendPlan p;
+    if (int rc = plan_attend(a.cache, a.batch, cache->head_dim, a.group, window, sinks, max_query_len ? max_query_len : a.batch.tokens,
+                             max_seq_len ? max_seq_len : a.batch.table_width << (a.cache.page_shift + 5), &p))
+        return rc;
+    if (p.work_bytes && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < p.work_bytes))
+        return fail(CI_ERR_CAPACITY, "%s: the workspace must be 16-byte aligned and hold %zu bytes", who, p.work_bytes);
+    if (int rc = device_status_word(&a.batch.status)) return rc;
+    a.work = static_cast<float *>(d_workspace);
+    a.whole = p.whole ? 1 : 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool wide = cache->head_dim == 128;
+    if (cache->kind == CI_KV_BF16) return wide ? launch_attend<CI_KV_BF16, 128>(a, p, s) : launch_attend<CI_KV_BF16, 64>(a, p, s);
+    return wide ? launch_attend<CI_KV_INT4, 128>(a, p, s) : launch_attend<CI_KV_INT4, 64>(a, p, s);
+}

@@ -48,6 +48,9 @@ inline uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
 inline bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// Device address of the current device's status word (ci_device_status).
+int device_status_word(uint32_t **word);
+
 // Largest LDS allocation a workgroup may ask for on gfx950 (160 KB per CU).
 constexpr uint32_t kLdsLimit = 160 * 1024;
 

@@ -1244,6 +1244,25 @@ static std::atomic<uint32_t> g_wait_limit{1u << 22};
 
 extern "C" uint32_t ci_debug_wait_limit(uint32_t looks) { return g_wait_limit.exchange(looks); }
 
+// The status word's address on the current device, for kernels of other sources that report to it (asked for once per
+// device: ci_check_device does it, outside any capture).
+namespace ci {
+int device_status_word(uint32_t **word) {
+    static std::atomic<uint32_t *> known[64];
+    int dev = 0;
+    CI_HIP(hipGetDevice(&dev));
+    uint32_t *w = known[dev & 63].load(std::memory_order_acquire);
+    if (!w) {
+        void *p = nullptr;
+        CI_HIP(hipGetSymbolAddress(&p, HIP_SYMBOL(g_device_status)));
+        w = static_cast<uint32_t *>(p);
+        known[dev & 63].store(w, std::memory_order_release);
+    }
+    *word = w;
+    return CI_OK;
+}
+}  // namespace ci
+
 extern "C" int ci_device_status(uint32_t *h_status, ci_stream_t stream) {
     if (!h_status) return fail(CI_ERR_ARG, "ci_device_status: null result pointer");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1252,7 +1271,10 @@ extern "C" int ci_device_status(uint32_t *h_status, ci_stream_t stream) {
     CI_HIP(hipMemcpyAsync(h_status, word, sizeof(uint32_t), hipMemcpyDeviceToHost, s));
     CI_HIP(hipMemsetAsync(word, 0, sizeof(uint32_t), s));
     CI_HIP(hipStreamSynchronize(s));
-    if (*h_status) return fail(CI_ERR_HIP, "a kernel gave up a bounded wait (device status 0x%x): results since the last check are not to be used", *h_status);
+    if (*h_status & CI_STATUS_WAIT_GAVE_UP)
+        return fail(CI_ERR_HIP, "a kernel gave up a bounded wait (device status 0x%x): results since the last check are not to be used", *h_status);
+    if (*h_status)
+        return fail(CI_ERR_HIP, "a batch of the paged cache named rows, tokens or pages that do not exist (device status 0x%x): they were left out", *h_status);
     return CI_OK;
 }
 

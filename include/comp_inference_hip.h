@@ -559,8 +559,89 @@ int ci_fused_linear_transposed_matrix_sums(int enable);
  *                        value.  0 makes every such wait give up at once: the give-up path under test.
  * ------------------------------------------------------------------------------------- */
 #define CI_STATUS_WAIT_GAVE_UP 1u
+#define CI_STATUS_BAD_INDEX 2u /* a batch of the paged cache named rows, tokens or pages that do not exist */
 int ci_device_status(uint32_t *h_status, ci_stream_t stream);
 uint32_t ci_debug_wait_limit(uint32_t looks);
+
+/* ---------------------------------------------------------------------------------------
+ * The paged key/value cache and attention over it: what stands between the compressed linears of a decoder.  No
+ * counterpart in the reference, whose models run the attention of the library they come from.
+ *
+ * ci_kv_cache: pages of `page_size` tokens for `kv_heads` heads of `head_dim` channels, keys and values in bf16 or in
+ * 4 bits, in the library's own order (comp_inference_amd/csrc/paged.h); one layer each.  A 4-bit row (one token, one
+ * head) is held as codes 0..15 with a bf16 pair: low = the row's minimum, step = (maximum - minimum) / 15 rounded up to
+ * bf16, code = (x - low) / step rounded to the nearest (ties to even); it stands for low + code * step.  A row with an
+ * infinity or a NaN reads back as NaN throughout.
+ *
+ * ci_kv_batch: sequences of which the last tokens are new.  d_query_start [num_seqs + 1] cuts the rows of q / k / v /
+ * out into sequences (NULL: one row each, in order, num_tokens == num_seqs); d_seq_lens [num_seqs] counts every
+ * sequence's tokens with the new ones; row b of d_block_table names the pages of sequence b, as many as its length
+ * needs, the entries behind them are not read.  All three lie on the device and are read by the kernels (a captured
+ * graph may be replayed with new contents).  Rows behind the last sequence are neither read nor written.  A place of a
+ * padded batch (no d_query_start, length 0) is left out by the cache operators and gets zeros from attention.
+ *   Two sequences of a call may share pages they only read; pages that a call appends to belong to one sequence.
+ *   Lengths, row offsets or pages outside the tensors are never followed: such tokens are left out (attention treats
+ *   them as not visible, appending stores nothing and writes no query row) and CI_STATUS_BAD_INDEX is recorded
+ *   (ci_device_status).
+ *
+ * ci_rows: bf16 [rows, heads, head_dim] with strides in elements (multiples of 8) and unit stride inside a head;
+ * 16-byte aligned.
+ *
+ *   ci_kv_cache_bytes    bytes of d_data; 0 for a shape that cannot be (head_dim 64 or 128; page_size a power of two
+ *                        from 32 to 4096; kv_heads up to 1024)
+ *   ci_paged_kv_append   stores k and v of the new tokens.  With d_rotary (fp32 [rotary_rows, rotary_dim]: cosines, then
+ *                        sines, of each position's rotary_dim / 2 angles) keys and, if given, queries are turned by
+ *                        their position's angles first: channels d and d + rotary_dim / 2 form a pair, channels from
+ *                        rotary_dim on stay.  The rotation is exact up to its one rounding to bf16.  q and q_out (both
+ *                        or neither; may be the same) hold q_heads heads.
+ *   ci_paged_kv_read     the stored keys and values of the last tokens of every sequence as rows
+ *   ci_paged_attention   out = softmax over the visible keys of scale * q k^T, times v: key j is visible to the query at
+ *                        position p when j <= p and (window == 0, or p - j < window, or j < sinks).  Query head h reads
+ *                        kv head h / (q_heads / kv_heads).  A row that sees no key gets zeros.  d_lse (or NULL): fp32
+ *                        [rows, q_heads], row stride lse_stride: natural logarithm of the sum of exp(scores), -inf for
+ *                        a row without keys.  max_query_len / max_seq_len: the caller's bounds on the lengths (0: not
+ *                        known); they choose kernels, the results do not rest on them.  The workspace is scratch of
+ *                        this call: ci_paged_attention_workspace_bytes says how much, for the same arguments.
+ * All are enqueued and not waited for, allocate nothing and may be captured.
+ * ------------------------------------------------------------------------------------- */
+#define CI_KV_BF16 0u
+#define CI_KV_INT4 1u
+
+typedef struct ci_kv_cache {
+    void *d_data;
+    uint64_t data_bytes;
+    uint32_t num_pages, page_size, kv_heads, head_dim, kind;
+} ci_kv_cache;
+
+typedef struct ci_kv_batch {
+    const int32_t *d_block_table; /* [num_seqs, table_width], rows table_stride elements apart */
+    uint32_t table_stride, table_width;
+    const int32_t *d_seq_lens;    /* [num_seqs] */
+    const int32_t *d_query_start; /* [num_seqs + 1] or NULL */
+    uint32_t num_seqs, num_tokens;
+} ci_kv_batch;
+
+typedef struct ci_rows {
+    void *d_data;
+    int64_t row_stride, head_stride;
+} ci_rows;
+
+uint64_t ci_kv_cache_bytes(uint32_t num_pages, uint32_t page_size, uint32_t kv_heads, uint32_t head_dim, uint32_t kind);
+
+int ci_paged_kv_append(const ci_kv_cache *cache, const ci_kv_batch *batch, const ci_rows *k, const ci_rows *v,
+                       const ci_rows *q, const ci_rows *q_out, uint32_t q_heads, const float *d_rotary,
+                       uint32_t rotary_rows, uint32_t rotary_dim, ci_stream_t stream);
+
+int ci_paged_kv_read(const ci_kv_cache *cache, const ci_kv_batch *batch, const ci_rows *k, const ci_rows *v,
+                     ci_stream_t stream);
+
+size_t ci_paged_attention_workspace_bytes(const ci_kv_cache *cache, const ci_kv_batch *batch, uint32_t q_heads,
+                                          int32_t window, int32_t sinks, uint32_t max_query_len, uint32_t max_seq_len);
+
+int ci_paged_attention(const ci_kv_cache *cache, const ci_kv_batch *batch, const ci_rows *q, const ci_rows *out,
+                       float *d_lse, int64_t lse_stride, uint32_t q_heads, float scale, int32_t window, int32_t sinks,
+                       uint32_t max_query_len, uint32_t max_seq_len, void *d_workspace, size_t workspace_bytes,
+                       ci_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Verification aids: the contraction of the fused kernels applied to a plain (uncompressed) bf16

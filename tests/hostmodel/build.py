@@ -39,7 +39,8 @@ ORDER_FLAGS = ["-fsanitize=thread", "-mllvm", "-tsan-instrument-func-entry-exit=
 UNDEFINED_LIB_PATH = os.path.join(HERE, "libci_hostmodel_undefined.so")
 UNDEFINED_FLAGS = ["-fsanitize=bounds,shift,alignment,integer-divide-by-zero,null,unreachable,signed-integer-overflow,pointer-overflow"]
 CXX = os.environ.get("CI_HOSTMODEL_CXX", "/opt/rocm/llvm/bin/clang++")
-SOURCES = ["api.hip", "encode.hip", "decode.hip", "linear.hip", "embedding.hip", "transposed.hip", "legacy.hip"]
+SOURCES = ["api.hip", "encode.hip", "decode.hip", "linear.hip", "embedding.hip", "transposed.hip", "legacy.hip",
+           "kv_cache.hip", "attention.hip"]
 CXXFLAGS = ["-std=c++17", "-O1", "-g", "-fPIC", "-fno-strict-aliasing", "-Wno-unused-value", "-Wno-unknown-attributes",
             "-Wno-ignored-attributes", "-Wno-pass-failed", "-Wno-psabi"]
 

@@ -74,6 +74,7 @@ CI_SIM_MINMAX(double)
 #define __builtin_amdgcn_wave_barrier() sim::wave_sync()
 #define __builtin_amdgcn_s_sleep(n) sim::yield()
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, x, y, z) sim::mfma_32x32x16_bf16((a), (b), (c))
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __shfl(v, src, width) sim::shfl((int)(v), (int)(src), (int)(width))
 #define __shfl_up(v, d, width) sim::shfl_up((int)(v), (unsigned)(d), (int)(width))
 
