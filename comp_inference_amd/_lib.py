@@ -104,7 +104,9 @@ def ptr(t: torch.Tensor | None) -> C.c_void_p:
 
 
 def stream_handle(device: torch.device) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """torch's current stream on `device` (the raw handle: making a Stream object around it costs microseconds)."""
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 def as_u32(t: torch.Tensor, device) -> torch.Tensor:

@@ -8,6 +8,7 @@ so a captured graph may be replayed with new contents.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -64,12 +65,23 @@ class PagedKVCache:
         per = nbytes // (self.num_pages * self.kv_heads * blocks * dtype.itemsize)
         self.data = torch.zeros(self.num_pages, self.kv_heads, blocks, per, dtype=dtype, device=device)
 
-    def _struct(self) -> _Cache:
+        self._bound = None
+
+    def _struct(self):
+        """The C descriptor by reference; made again when `data` is another memory."""
         d = self.data
-        if not d.is_contiguous():
-            raise RuntimeError("the cache's data must stay contiguous")
-        return _Cache(d.data_ptr(), d.numel() * d.element_size(), self.num_pages, self.page_size, self.kv_heads,
-                      self.head_dim, KINDS[self.kind])
+        at = d.data_ptr()
+        if self._bound is None or self._bound[0] != at or not d.is_contiguous():
+            if not d.is_contiguous():
+                raise RuntimeError("the cache's data must stay contiguous")
+            c = _Cache(at, d.numel() * d.element_size(), self.num_pages, self.page_size, self.kv_heads, self.head_dim,
+                       KINDS[self.kind])
+            self._bound = (at, c, C.byref(c))
+        return self._bound[2]
+
+    # A copy (copy.deepcopy, pickling) has memory of its own: the descriptor is made again there.
+    def __getstate__(self):
+        return {**self.__dict__, "_bound": None}
 
 
 def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -82,48 +94,65 @@ def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, device
     return torch.cat((angle.cos(), angle.sin()), dim=1).to(torch.float32).to(device)
 
 
-def _on(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise RuntimeError(f"{name} is on {t.device}, the cache on {device}")
+def _elsewhere(name: str, t, cache: PagedKVCache):
+    return RuntimeError(f"{name} is on {t.device}, the cache on {cache.data.device}")
 
 
-def _batch(cache: PagedKVCache, block_table, seq_lens, query_start, tokens: int) -> _Batch:
-    _on(cache.data.device, block_table=block_table, seq_lens=seq_lens, query_start=query_start)
+def _batch(cache: PagedKVCache, index: int, block_table, seq_lens, query_start, tokens: int):
+    """ci_kv_batch by reference.  (These checks run in front of every launch of a token loop: one query per property.)"""
+    seqs, width = seq_lens.numel(), 0
     for name, t, dim in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1), ("query_start", query_start, 1)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != dim):
+        if t is None:
+            continue
+        if t.dtype is not torch.int32 or t.dim() != dim:
             raise RuntimeError(f"{name} must be a {dim}-D int32 tensor")
-    seqs = seq_lens.numel()
-    if block_table.shape[0] != seqs or (query_start is not None and query_start.numel() != seqs + 1):
+        if t.get_device() != index:
+            raise _elsewhere(name, t, cache)
+    rows, width = block_table.shape
+    if rows != seqs or (query_start is not None and query_start.numel() != seqs + 1):
         raise ValueError(f"block_table must have {seqs} rows and query_start {seqs + 1} entries for {seqs} sequences")
     if query_start is None and tokens != seqs:
         raise ValueError(f"without query_start there is one new token per sequence: {tokens} rows, {seqs} sequences")
+    step, inner = block_table.stride()
     if seqs and (not seq_lens.is_contiguous() or (query_start is not None and not query_start.is_contiguous())
-                 or (block_table.shape[1] > 1 and block_table.stride(1) != 1) or block_table.stride(0) < 0):
+                 or (width > 1 and inner != 1) or step < 0):
         raise RuntimeError("seq_lens and query_start must be contiguous, and the rows of block_table")
-    width = block_table.shape[1]
-    return _Batch(block_table.data_ptr(), block_table.stride(0) if seqs > 1 else width, width, seq_lens.data_ptr(),
-                  None if query_start is None else query_start.data_ptr(), seqs, tokens)
+    return C.byref(_Batch(block_table.data_ptr(), step if seqs > 1 else width, width, seq_lens.data_ptr(),
+                          None if query_start is None else query_start.data_ptr(), seqs, tokens))
 
 
-def _rows(name: str, t: torch.Tensor, device, heads: int | None, dim: int, tokens: int | None) -> _Rows:
-    """[tokens, heads, dim] in bf16 with unit stride inside a head."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3:
+def _rows(name: str, t: torch.Tensor, cache: PagedKVCache, index: int, heads: int | None, tokens: int | None):
+    """ci_rows by reference of [tokens, heads, head_dim] in bf16 with unit stride inside a head."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3:
         raise RuntimeError(f"{name} must be a 3-D bfloat16 tensor [tokens, heads, head_dim]")
-    _on(device, **{name: t})
-    if t.shape[2] != dim or (heads is not None and t.shape[1] != heads) or (tokens is not None and t.shape[0] != tokens):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}; the other operands ask for ({tokens}, {heads}, {dim})")
-    if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or t.stride(0) % 8 or t.stride(1) % 8):
+    if t.get_device() != index:
+        raise _elsewhere(name, t, cache)
+    n, h, d = t.shape
+    if d != cache.head_dim or (heads is not None and h != heads) or (tokens is not None and n != tokens):
+        raise ValueError(f"{name} has shape {(n, h, d)}; the other operands ask for ({tokens}, {heads}, {cache.head_dim})")
+    at, (row, head, inner) = t.data_ptr(), t.stride()
+    if (inner != 1 or at % 16 or row % 8 or head % 8) and t.numel():
         raise RuntimeError(f"{name} must have unit stride inside a head, 16-byte aligned rows and strides that are multiples of 8")
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+    return C.byref(_Rows(at, row, head))
 
 
-def _output(name: str, given, tokens: int, heads: int, dim: int, device) -> torch.Tensor:
+def _output(name: str, given, tokens: int, heads: int, cache: PagedKVCache) -> torch.Tensor:
     if given is None:
-        return torch.empty(tokens, heads, dim, dtype=torch.bfloat16, device=device)
-    if given.numel() and tokens > 1 and given.dim() == 3 and (given.stride(0) == 0 or (heads > 1 and given.stride(1) == 0)):
-        raise RuntimeError(f"{name} must not overlap itself")
+        return torch.empty((tokens, heads, cache.head_dim), dtype=torch.bfloat16, device=cache.data.device)
+    if given.dim() == 3 and given.numel():
+        # (the strides that are used must lead from one head to another place)
+        steps = sorted((s, n) for s, n in zip(given.stride(), given.shape) if n > 1)
+        if any(s < (steps[i - 1][0] * steps[i - 1][1] if i else 1) for i, (s, _) in enumerate(steps)):
+            raise RuntimeError(f"{name} must not overlap itself")
     return given
+
+
+def _here(index: int):
+    """The context in which kernels of device `index` are launched (none where it is the current one already)."""
+    return _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 def paged_kv_append(cache: PagedKVCache, k, v, block_table, seq_lens, query_start=None, q=None, rotary=None, q_out=None):
@@ -135,29 +164,34 @@ def paged_kv_append(cache: PagedKVCache, k, v, block_table, seq_lens, query_star
     sequences of length 0, are left as they were.  Tokens, pages and table rows that do not exist are left out and
     reported by `device_status`."""
     _lib.require_device(cache.data)
-    dev, H, D = cache.data.device, cache.kv_heads, cache.head_dim
-    tokens = k.shape[0] if k.dim() else 0
-    kr, vr = _rows("k", k, dev, H, D, None), _rows("v", v, dev, H, D, tokens)
-    b = _batch(cache, block_table, seq_lens, query_start, tokens)
+    index, H = cache.data.get_device(), cache.kv_heads
+    kr = _rows("k", k, cache, index, H, None)
+    tokens = k.shape[0]
+    vr = _rows("v", v, cache, index, H, tokens)
+    b = _batch(cache, index, block_table, seq_lens, query_start, tokens)
     qr = orows = None
+    heads = positions = turned = 0
+    table = None
     if q is not None:
-        qr = _rows("q", q, dev, None, D, tokens)
-        q_out = _output("q_out", q_out, tokens, q.shape[1], D, dev)
-        orows = _rows("q_out", q_out, dev, q.shape[1], D, tokens)
+        qr = _rows("q", q, cache, index, None, tokens)
+        heads = q.shape[1]
+        q_out = _output("q_out", q_out, tokens, heads, cache)
+        orows = _rows("q_out", q_out, cache, index, heads, tokens)
     elif q_out is not None:
         raise ValueError("q_out without q")
     if rotary is not None:
-        _on(dev, rotary=rotary)
-        if rotary.dtype != torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous():
+        if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous():
             raise RuntimeError("rotary must be a contiguous 2-D float32 tensor [positions, rotary_dim]")
-        if rotary.shape[1] == 0 or rotary.shape[1] % 16 or rotary.shape[1] > D:
-            raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim, not {rotary.shape[1]}")
+        if rotary.get_device() != index:
+            raise _elsewhere("rotary", rotary, cache)
+        positions, turned = rotary.shape
+        if turned == 0 or turned % 16 or turned > cache.head_dim:
+            raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim, not {turned}")
+        table = C.c_void_p(rotary.data_ptr())
     c = cache._struct()
-    with torch.cuda.device(dev):
-        check(lib().ci_paged_kv_append(
-            C.byref(c), C.byref(b), C.byref(kr), C.byref(vr), None if qr is None else C.byref(qr),
-            None if orows is None else C.byref(orows), 0 if q is None else q.shape[1], ptr(rotary),
-            0 if rotary is None else rotary.shape[0], 0 if rotary is None else rotary.shape[1], _lib.stream_handle(dev)))
+    with _here(index):
+        check(lib().ci_paged_kv_append(c, b, kr, vr, qr, orows, heads, table, positions, turned,
+                                       _lib.stream_handle(cache.data.device)))
     return q_out
 
 
@@ -166,18 +200,18 @@ def paged_kv_read(cache: PagedKVCache, block_table, seq_lens, query_start=None, 
     `query_start` cuts the rows as for `paged_kv_append`.  `tokens`: rows in all (needed with `query_start` unless the
     outputs are given; reading it from the device would wait for it)."""
     _lib.require_device(cache.data)
-    dev, H, D = cache.data.device, cache.kv_heads, cache.head_dim
+    index, H = cache.data.get_device(), cache.kv_heads
     if tokens is None:
         if query_start is not None and k_out is None:
             raise ValueError("tokens (the number of rows) is needed with query_start")
         tokens = seq_lens.numel() if query_start is None else k_out.shape[0]
     tokens = int(tokens)
-    k_out, v_out = _output("k_out", k_out, tokens, H, D, dev), _output("v_out", v_out, tokens, H, D, dev)
-    kr, vr = _rows("k_out", k_out, dev, H, D, tokens), _rows("v_out", v_out, dev, H, D, tokens)
-    b = _batch(cache, block_table, seq_lens, query_start, tokens)
+    k_out, v_out = _output("k_out", k_out, tokens, H, cache), _output("v_out", v_out, tokens, H, cache)
+    kr, vr = _rows("k_out", k_out, cache, index, H, tokens), _rows("v_out", v_out, cache, index, H, tokens)
+    b = _batch(cache, index, block_table, seq_lens, query_start, tokens)
     c = cache._struct()
-    with torch.cuda.device(dev):
-        check(lib().ci_paged_kv_read(C.byref(c), C.byref(b), C.byref(kr), C.byref(vr), _lib.stream_handle(dev)))
+    with _here(index):
+        check(lib().ci_paged_kv_read(c, b, kr, vr, _lib.stream_handle(cache.data.device)))
     return k_out, v_out
 
 
@@ -191,28 +225,30 @@ def paged_attention(q, cache: PagedKVCache, block_table, seq_lens, query_start=N
     also fp32 [T, heads], the natural logarithm of the sum of exp(scores).  Scores, sums and the output are held in 32
     bits; the weights are rounded to bf16 for the product with v.  Inference only."""
     _lib.require_device(cache.data)
-    dev, D = cache.data.device, cache.head_dim
-    qr = _rows("q", q, dev, None, D, None)
+    dev = cache.data.device
+    index = cache.data.get_device()
+    qr = _rows("q", q, cache, index, None, None)
     tokens, heads = q.shape[0], q.shape[1]
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
-    out = _output("out", out, tokens, heads, D, dev)
-    orows = _rows("out", out, dev, heads, D, tokens)
-    b = _batch(cache, block_table, seq_lens, query_start, tokens)
+    out = _output("out", out, tokens, heads, cache)
+    orows = _rows("out", out, cache, index, heads, tokens)
+    b = _batch(cache, index, block_table, seq_lens, query_start, tokens)
     limit = (1 << 31) - 1
-    if not (0 <= int(window) <= limit and 0 <= int(sinks) <= limit):
+    window, sinks = int(window), int(sinks)
+    if not (0 <= window <= limit and 0 <= sinks <= limit):
         raise ValueError("window and sinks must be 0 to 2^31 - 1")
-    max_query_len, max_seq_len = (min(max(int(x), 0), limit) for x in (max_query_len, max_seq_len))
+    max_query_len, max_seq_len = min(max(int(max_query_len), 0), limit), min(max(int(max_seq_len), 0), limit)
     lse = torch.empty(tokens, heads, dtype=torch.float32, device=dev) if return_lse else None
     c = cache._struct()
-    fn = lib().ci_paged_attention_workspace_bytes
-    fn.restype = C.c_size_t
-    with torch.cuda.device(dev):
-        need = fn(C.byref(c), C.byref(b), heads, int(window), int(sinks), max_query_len, max_seq_len)
+    library = lib()
+    library.ci_paged_attention_workspace_bytes.restype = C.c_size_t
+    with _here(index):
+        need = library.ci_paged_attention_workspace_bytes(c, b, heads, window, sinks, max_query_len, max_seq_len)
         # (a workspace of the call's own: two captured graphs never share one)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(lib().ci_paged_attention(
-            C.byref(c), C.byref(b), C.byref(qr), C.byref(orows), ptr(lse), C.c_int64(heads), heads,
-            C.c_float(D ** -0.5 if scale is None else float(scale)), int(window), int(sinks), max_query_len, max_seq_len,
+        check(library.ci_paged_attention(
+            c, b, qr, orows, ptr(lse), C.c_int64(heads), heads,
+            C.c_float(cache.head_dim ** -0.5 if scale is None else float(scale)), window, sinks, max_query_len, max_seq_len,
             ptr(ws), C.c_size_t(need), _lib.stream_handle(dev)))
     return (out, lse) if return_lse else out

@@ -527,6 +527,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
     __shared__ uint32_t word[8];
     __shared__ float part[256 * 4];
     __shared__ float part_l[16];
+    __shared__ float part_m[16];
     Item it;
     if (!find_item<RP>(a, blockIdx.x, word, it)) return;
     bool bad;
@@ -554,32 +555,54 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
     before += it.head * units;
     const uint32_t share = share_of(total, workers), w0 = before / share, w1 = (before + units - 1) / share;
     if (w0 == w1) return;  // (written whole)
+    // every group of threads takes each kGroups-th part, four of them asked for at a time, with a maximum of its own
     const uint32_t g = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
-    float m = kNone;
-    for (uint32_t w = w0; w <= w1; ++w)
-        m = fmaxf(m, a.work[(uint64_t)(w * 2 + (w == w0 ? 1 : 0)) * slot_floats<D, RP>() + RP * D + row]);
+    float m = kNone, l = 0.0f;
     f32x4_p acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-    for (uint32_t w = w0 + g; w <= w1; w += kGroups) {
-        const float *slot = a.work + (uint64_t)(w * 2 + (w == w0 ? 1 : 0)) * slot_floats<D, RP>();
-        const float mw = slot[RP * D + row], f = mw == kNone ? 0.0f : exp2_fast(mw - m);
-        const f32x4_p y = *reinterpret_cast<const f32x4_p *>(slot + row * D + d);
-        l += f * slot[RP * D + RP + row];
+    for (uint32_t w = w0 + g; w <= w1; w += 4 * kGroups) {
+        float mw[4], lw[4];
+        f32x4_p y[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
+        for (uint32_t k = 0; k < 4; ++k) {  // (past the last part: the last one again, with no weight)
+            const uint32_t at = min(w + k * kGroups, w1);
+            const float *slot = a.work + (uint64_t)(at * 2 + (at == w0 ? 1 : 0)) * slot_floats<D, RP>();
+            mw[k] = slot[RP * D + row];
+            lw[k] = slot[RP * D + RP + row];
+            y[k] = *reinterpret_cast<const f32x4_p *>(slot + row * D + d);
+        }
+        float top = m;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) top = fmaxf(top, mw[k]);
+        const float f0 = m == kNone ? 0.0f : exp2_fast(m - top);
+        l *= f0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] *= f0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            if (w + k * kGroups > w1) continue;
+            const float f = mw[k] == kNone ? 0.0f : exp2_fast(mw[k] - top);
+            l += f * lw[k];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] += f * y[k][c];
+        }
+        m = top;
     }
     *reinterpret_cast<f32x4_p *>(part + threadIdx.x * 4) = acc;
-    if (d == 0) part_l[g] = l;
+    if (d == 0) part_l[g] = l, part_m[g] = m;
     __syncthreads();
     if (threadIdx.x >= kLanes) return;
+    m = kNone;
+#pragma unroll
+    for (uint32_t k = 0; k < kGroups; ++k) m = fmaxf(m, part_m[k]);
     l = 0.0f;
     acc = f32x4_p{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (uint32_t k = 0; k < kGroups; ++k) {
-        l += part_l[k];
+        const float f = part_m[k] == kNone ? 0.0f : exp2_fast(part_m[k] - m);
+        l += f * part_l[k];
         const f32x4_p y = *reinterpret_cast<const f32x4_p *>(part + (k * kLanes + threadIdx.x) * 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] += y[c];
+        for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     const uint32_t tok = (r0 + row) / a.group, gh = it.head * a.group + (r0 + row) % a.group;
