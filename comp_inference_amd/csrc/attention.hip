@@ -41,6 +41,9 @@ constexpr uint32_t kUnit = 4;  // blocks of a unit of work: one per wavefront
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// (one instruction for three operands, and none to quiet a NaN first: a NaN among scores is carried by their weights)
+__device__ __forceinline__ float most(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
 __device__ __forceinline__ float other_half(float x) {  // the value of lane ^ 32
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
@@ -355,7 +358,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             if (KIND != CI_KV_BF16) t[e] = t[e] * bf16_lo(kp[e]) + q.sum * bf16_hi(kp[e]);
             t[e] *= a.scale_log2;
             if (edge) t[e] = sees >> ((e & 3) + 8 * (e >> 2)) & 1 ? t[e] : kNone;
-            best = fmaxf(best, t[e]);
+            best = most(best, t[e]);
         }
         run.raise(max_halves(best));
         const float base = run.base();
@@ -620,6 +623,9 @@ constexpr uint32_t rows_lds(int D) { return 2 * 2 * 128 * D; }  // two buffers o
 template <int KIND, int D>
 struct Stage;
 
+// The keys behind the end of a sequence need not be numbers; their scores are set, and their values are put to zero here.
+// `held` has a bit for every token of the block that is there (all ones: nothing to do).
+
 // bf16: blocks are copied as they lie.
 template <int D>
 struct Stage<CI_KV_BF16, D> {
@@ -630,7 +636,16 @@ struct Stage<CI_KV_BF16, D> {
         for (int i = 0; i < N; ++i)
             x[i] = reinterpret_cast<const u32x4 *>(i < N / 2 ? b0 : b1)[(i % (N / 2)) * 256 + threadIdx.x];
     }
-    __device__ __forceinline__ void store(uint8_t *lds) const {
+    __device__ __forceinline__ void store(uint8_t *lds, uint32_t held0, uint32_t held1) {
+        if ((held0 & held1) != 0xFFFFFFFFu) {
+            const uint32_t h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (i % (N / 2) < N / 4) continue;  // (keys)
+                const uint32_t o = (i % (N / 4)) * 256 + threadIdx.x, held = i < N / 2 ? held0 : held1;
+                x[i] = keep_seen(x[i], held >> (16 * (o / (2 * D)) + 4 * h), 0);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) reinterpret_cast<u32x4 *>(lds)[i * 256 + threadIdx.x] = x[i];
     }
@@ -664,8 +679,9 @@ struct Stage<CI_KV_INT4, D> {
             if (!values) pair[u * 8] = key;
         }
     }
-    __device__ __forceinline__ void store(uint8_t *lds) const {
+    __device__ __forceinline__ void store(uint8_t *lds, uint32_t held0, uint32_t held1) const {
         const uint32_t lane = threadIdx.x & 63;
+        const bool tail = (held0 & held1) != 0xFFFFFFFFu;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
@@ -682,6 +698,8 @@ struct Stage<CI_KV_INT4, D> {
                     y[w] = bf16_pair(fmaf(bf16_lo(p0), bf16_lo(n[w]) - 128.0f, bf16_hi(p0)),
                                      fmaf(bf16_lo(p1), bf16_hi(n[w]) - 128.0f, bf16_hi(p1)));
                 }
+                if (tail && values)
+                    y = keep_seen(y, (blk ? held1 : held0) >> (4 * (lane >> 5) + 16 * (U == 2 ? i : c / 2)), 0);
                 dst[(i * 4 + c) * 64 + lane] = y;
             }
         }
@@ -733,22 +751,24 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         const uint8_t *b0 = place(0, gone[0]), *b1 = place(1, gone[1]);
         stage.fetch(b0, b1);
     }
+    const auto held = [&](int32_t kb, bool g) { return g ? 0u : bits(0, s.len - kb); };
     for (uint32_t st = 0; st < steps; ++st) {
         uint8_t *buf = lds + (st & 1) * (256 * D);
-        stage.store(buf);
         const bool g0 = gone[0], g1 = gone[1] || 2 * st + 1 >= span.nb;
+        const int32_t kb0 = (int32_t)(span.block(2 * st) * kKvBlock);
+        const int32_t kb1 = (int32_t)(span.block(min(2 * st + 1, span.nb - 1)) * kKvBlock);
+        stage.store(buf, held(kb0, g0), held(kb1, g1));
         lost = lost || g0 || gone[1];
         __syncthreads();
         if (st + 1 < steps) {
             const uint8_t *b0 = place(2 * st + 2, gone[0]), *b1 = place(2 * st + 3, gone[1]);
             stage.fetch(b0, b1);
         }
-        const int32_t kb0 = (int32_t)(span.block(2 * st) * kKvBlock);
-        const int32_t kb1 = (int32_t)(span.block(min(2 * st + 1, span.nb - 1)) * kKvBlock);
         // a wavefront none of whose rows sees a key of either block has nothing to do in this step
         const int32_t lo = a.window ? own.p_lo - a.window + 1 : 0;
         const auto seen = [&](int32_t kb) { return kb <= own.p_hi && (kb + 31 >= lo || kb < a.sinks); };
         if (!any || !((seen(kb0) && !g0) || (seen(kb1) && !g1))) continue;
+        const bool edge = g0 || g1 || !all_visible(a, own, kb0) || !all_visible(a, own, kb1);
 
         const u32x4 *kv = reinterpret_cast<const u32x4 *>(buf);
         constexpr int kBlk = 8 * D;  // 16-byte pieces of a block: keys, then values
@@ -758,8 +778,6 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
             acc0 = mfma(kv[k * 64 + lane], q.f[k], acc0);
             acc1 = mfma(kv[kBlk + k * 64 + lane], q.f[k], acc1);
         }
-        const bool edge = g0 || g1 || !all_visible(a, own, kb0) || !all_visible(a, own, kb1);
-        uint32_t seen0 = 0, seen1 = 0;  // of the wavefront's rows, from key 4 h on
         if (edge) {
             const uint32_t s0 = g0 ? 0u : seen_keys(a, pos, pos, kb0) >> (4 * h), s1 = g1 ? 0u : seen_keys(a, pos, pos, kb1) >> (4 * h);
 #pragma unroll
@@ -767,12 +785,10 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
                 acc0[e] = s0 >> ((e & 3) + 8 * (e >> 2)) & 1 ? acc0[e] : kNone;
                 acc1[e] = s1 >> ((e & 3) + 8 * (e >> 2)) & 1 ? acc1[e] : kNone;
             }
-            seen0 = g0 ? 0u : seen_keys(a, own.p_lo, own.p_hi, kb0) >> (4 * h);
-            seen1 = g1 ? 0u : seen_keys(a, own.p_lo, own.p_hi, kb1) >> (4 * h);
         }
         float best = kNone;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) best = fmaxf(best, fmaxf(acc0[e], acc1[e]));
+        for (int e = 0; e < 16; ++e) best = most(best, most(acc0[e], acc1[e]));
         run.raise(max_halves(best) * a.scale_log2);
         const float base = run.base();
         u32x4 p[4];
@@ -787,11 +803,8 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
 #pragma unroll
         for (int s2 = 0; s2 < 4; ++s2)
 #pragma unroll
-            for (int db = 0; db < D / 32; ++db) {
-                u32x4 v = kv[(s2 / 2) * kBlk + 4 * D + ((s2 % 2) * (D / 32) + db) * 64 + lane];
-                if (edge) v = keep_seen(v, s2 < 2 ? seen0 : seen1, s2 % 2);
-                run.o[db] = mfma(v, p[s2], run.o[db]);
-            }
+            for (int db = 0; db < D / 32; ++db)
+                run.o[db] = mfma(kv[(s2 / 2) * kBlk + 4 * D + ((s2 % 2) * (D / 32) + db) * 64 + lane], p[s2], run.o[db]);
     }
     if (lost && threadIdx.x == 0) report_bad_index(a.batch);
     const float l = run.l + other_half(run.l), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
