@@ -30,6 +30,7 @@ struct AttendArgs {
     float *lse;  // or nullptr: ln of the sum of exp(scores), [row, head]
     int64_t q_row, q_head, o_row, o_head, l_row;
     uint32_t group;  // query heads of a kv head
+    double per_group;  // 1 / group
     float scale_log2;  // scale * log2(e): the kernel works on powers of two
     int32_t window, sinks;  // window 0: none
     float *work;            // partial sums of cut items
@@ -56,6 +57,13 @@ __device__ __forceinline__ float max_halves(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// row / group, exact: the quotient of row + 1/2 is at least 1 / (2 group) >= 2^-17 away from the next whole number, and the
+// product is off by less than 2^-20 (rows are below 2^31).
+__device__ __forceinline__ uint32_t token_of(const AttendArgs &a, uint32_t row) {
+    return (uint32_t)(((double)row + 0.5) * a.per_group);
+}
+__device__ __forceinline__ uint32_t rows_of(const AttendArgs &a, const SeqInfo &s) { return (uint32_t)s.n * a.group; }
+
 // Rows [r0, r1) of a sequence, and the blocks of keys some of them see: [0, s1) and [w0, w0 + nb - s1).
 struct Span {
     int32_t p_lo, p_hi;  // positions of the first and last row
@@ -65,8 +73,8 @@ struct Span {
 
 __device__ __forceinline__ Span span_of(const AttendArgs &a, const SeqInfo &s, uint32_t r0, uint32_t r1) {
     Span x;
-    x.p_lo = s.len - s.n + (int32_t)(r0 / a.group);
-    x.p_hi = s.len - s.n + (int32_t)((r1 - 1) / a.group);
+    x.p_lo = s.len - s.n + (int32_t)token_of(a, r0);
+    x.p_hi = s.len - s.n + (int32_t)token_of(a, r1 - 1);
     const uint32_t end = x.p_hi < 0 ? 0 : (uint32_t)x.p_hi / kKvBlock + 1;
     x.s1 = x.w0 = 0;
     if (a.window) {
@@ -94,7 +102,6 @@ __device__ __forceinline__ uint32_t seen_keys(const AttendArgs &a, int32_t p_lo,
     return bits(p_lo - a.window + 1 - kb, p_hi + 1 - kb) | bits(0, min(a.sinks, p_hi + 1) - kb);
 }
 
-__device__ __forceinline__ uint32_t rows_of(const AttendArgs &a, const SeqInfo &s) { return (uint32_t)s.n * a.group; }
 
 // ---- matrix operands ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ f32x16_p mfma(u32x4 x, u32x4 y, f32x16_p c) {
@@ -126,7 +133,7 @@ __device__ __forceinline__ Queries<D> load_queries(const AttendArgs &a, const Se
     Queries<D> q;
     const uint32_t h = (threadIdx.x >> 5) & 1;
     const bool there = row < rows;
-    const uint32_t tok = there ? row / a.group : 0, g = there ? row % a.group : 0;
+    const uint32_t tok = there ? token_of(a, row) : 0, g = there ? row - tok * a.group : 0;
     const uint16_t *src = a.q + (int64_t)(s.row + (int32_t)tok) * a.q_row + (int64_t)(head * a.group + g) * a.q_head;
     q.sum = 0.0f;
 #pragma unroll
@@ -294,7 +301,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
     const Cols<RP> cols;
     const uint32_t row = col % RP;
     const Queries<D> q = load_queries<D>(a, s, it.head, r0 + row, r0 + rows);
-    const int32_t pos = s.len - s.n + (int32_t)((r0 + row) / a.group);
+    const int32_t pos = s.len - s.n + (int32_t)token_of(a, r0 + row);
     Running<D> run;
     run.clear();
     const f32x16_p start = splat16(KIND == CI_KV_BF16 ? 0.0f : -128.0f * q.sum);
@@ -446,7 +453,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
         }
         if (whole) {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing: zeros)
-            const uint32_t tok = (r0 + rr) / a.group, g = (r0 + rr) % a.group;
+            const uint32_t tok = token_of(a, r0 + rr), g = r0 + rr - tok * a.group;
             u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
             *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row +
                                        (int64_t)(it.head * a.group + g) * a.o_head + d) = w;
@@ -527,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void attend_split_kernel(AttendArgs a) {
 template <int D, int RP>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t workers) {
     constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
-    __shared__ uint32_t word[8];
+    __shared__ uint32_t word[10];
     __shared__ float part[256 * 4];
     __shared__ float part_l[16];
     __shared__ float part_m[16];
@@ -544,13 +551,13 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
         const uint32_t end = min(first + per, a.batch.seqs);
         uint32_t mine = 0;
         for (uint32_t i = first; i < end; ++i) mine += weight_of<RP>(a, i);
-        before = scan256(mine, word, total);
+        before = scan_threads(mine, word, total);
         if (it.seq >= first && it.seq < end) {
             for (uint32_t i = first; i < it.seq; ++i) before += weight_of<RP>(a, i);
-            word[6] = before;
+            word[8] = before;
         }
         __syncthreads();
-        before = uniform(word[6]);
+        before = uniform(word[8]);
         total = uniform(total);
     }
     for (uint32_t t = 0; t < it.tile; ++t) before += units_of<RP>(a, s, t) * a.cache.kv_heads;
@@ -608,7 +615,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
         for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const uint32_t tok = (r0 + row) / a.group, gh = it.head * a.group + (r0 + row) % a.group;
+    const uint32_t tok = token_of(a, r0 + row), gh = it.head * a.group + r0 + row - tok * a.group;
     u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
     *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
     if (a.lse && d == 0)
@@ -616,8 +623,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------
-constexpr uint32_t kTileRows = 128;  // four wavefronts of 32
+constexpr uint32_t kRowWaves = 8, kRowThreads = 64 * kRowWaves, kTileRows = 32 * kRowWaves;
 constexpr uint32_t rows_lds(int D) { return 2 * 2 * 128 * D; }  // two buffers of two blocks, keys and values in bf16
+constexpr uint32_t kLeastShare = 16;                             // steps (of 64 keys) worth a workgroup
 
 // What a thread carries of the next step from memory to the LDS.
 template <int KIND, int D>
@@ -629,54 +637,56 @@ struct Stage;
 // bf16: blocks are copied as they lie.
 template <int D>
 struct Stage<CI_KV_BF16, D> {
-    static constexpr int N = D / 16;  // 16-byte pieces per thread: 2 blocks x 128 D bytes / 4096
+    static constexpr int N = 256 * D / (16 * kRowThreads);  // 16-byte pieces per thread of two blocks of 128 D bytes
     u32x4 x[N];
+    static __device__ __forceinline__ uint32_t piece(int i) { return i * kRowThreads + threadIdx.x; }
     __device__ __forceinline__ void fetch(const uint8_t *b0, const uint8_t *b1) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            x[i] = reinterpret_cast<const u32x4 *>(i < N / 2 ? b0 : b1)[(i % (N / 2)) * 256 + threadIdx.x];
+            x[i] = reinterpret_cast<const u32x4 *>(i < N / 2 ? b0 : b1)[piece(i % (N / 2))];
     }
     __device__ __forceinline__ void store(uint8_t *lds, uint32_t held0, uint32_t held1) {
         if ((held0 & held1) != 0xFFFFFFFFu) {
             const uint32_t h = (threadIdx.x >> 5) & 1;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                if (i % (N / 2) < N / 4) continue;  // (keys)
-                const uint32_t o = (i % (N / 4)) * 256 + threadIdx.x, held = i < N / 2 ? held0 : held1;
-                x[i] = keep_seen(x[i], held >> (16 * (o / (2 * D)) + 4 * h), 0);
+                const uint32_t at = piece(i % (N / 2)), held = i < N / 2 ? held0 : held1;
+                if (at < 4 * D) continue;  // (keys)
+                x[i] = keep_seen(x[i], held >> (16 * ((at - 4 * D) / (2 * D)) + 4 * h), 0);
             }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) reinterpret_cast<u32x4 *>(lds)[i * 256 + threadIdx.x] = x[i];
+        for (int i = 0; i < N; ++i) reinterpret_cast<u32x4 *>(lds)[piece(i)] = x[i];
     }
 };
 
 // 4 bits: the codes become the values they stand for, rounded to bf16 (what a bf16 cache would hold of them), once for the
-// four wavefronts that use them.  A wavefront takes whole 1 KB pieces: for heads of 128 keys (wavefronts 0, 1) or values
-// (2, 3) of both blocks, for heads of 64 keys or values of one block.
+// wavefronts that use them.  A wavefront takes whole 1 KB pieces of codes, keys or values of one block.
 template <int D>
 struct Stage<CI_KV_INT4, D> {
-    static constexpr int N = D / 64, U = N;  // pieces of the keys of a block; pieces per wavefront: 2 * 2 * N / 4
+    static constexpr int N = D / 64;                                      // pieces of the keys of a block
+    static constexpr int U = 4 * N > (int)kRowWaves ? 4 * N / kRowWaves : 1;  // pieces per wavefront
     u32x4 x[U];
-    uint32_t pair[16];
-    static __device__ __forceinline__ uint32_t unit(int u) { return uniform(threadIdx.x >> 6) + 4 * u; }
+    uint32_t pair[U * 16 / N];  // (step, low): of the lane's key, or of its tokens (16 for heads of 64, 8 for 128)
+    static __device__ __forceinline__ uint32_t unit(int u) { return uniform(threadIdx.x >> 6) + kRowWaves * u; }
     __device__ __forceinline__ void fetch(const uint8_t *b0, const uint8_t *b1) {
         const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (unit(u) >= 4 * N) continue;
             const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
             const uint8_t *b = blk ? b1 : b0;
             x[u] = reinterpret_cast<const u32x4 *>(b + values * KvBlock<CI_KV_INT4, D>::kHalf)[i * 64 + lane];
             const uint32_t *p = reinterpret_cast<const uint32_t *>(b + KvBlock<CI_KV_INT4, D>::kPairs);
             const uint32_t key = p[lane & 31];
 #pragma unroll
-            for (int c = 0; c < 16 / U; c += 4) {  // tokens 16 s + 8 a + 4 h + b, s = i for heads of 128
-                const uint32_t s = U == 2 ? i : c / 8;
+            for (int c = 0; c < 16 / N; c += 4) {  // tokens 16 s + 8 a + 4 h + b, s = i for heads of 128
+                const uint32_t s = N == 2 ? i : c / 8;
                 const u32x4 w = *reinterpret_cast<const u32x4 *>(p + kKvBlock + 16 * s + 8 * (c / 4 % 2) + 4 * h);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) pair[u * 8 + c + e] = w[e];
+                for (int e = 0; e < 4; ++e) pair[u * 16 / N + c + e] = w[e];
             }
-            if (!values) pair[u * 8] = key;
+            if (!values) pair[u * 16 / N] = key;
         }
     }
     __device__ __forceinline__ void store(uint8_t *lds, uint32_t held0, uint32_t held1) const {
@@ -684,75 +694,123 @@ struct Stage<CI_KV_INT4, D> {
         const bool tail = (held0 & held1) != 0xFFFFFFFFu;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (unit(u) >= 4 * N) continue;
             const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
             u32x4 *dst = reinterpret_cast<u32x4 *>(lds + blk * 128 * D + values * 64 * D);
+            const uint32_t key = pair[u * 16 / N];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const u32x4 n = codes_to_bf16(x[u][c]);  // 128 + code
+                // codes 0, 4, 1, 5 and 2, 6, 3, 7 of the operand, a byte each
+                const uint32_t even = x[u][c] & 0x0F0F0F0Fu, odd = x[u][c] >> 4 & 0x0F0F0F0Fu;
                 u32x4 y;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const int at = u * 8 + (U == 2 ? 0 : c / 2 * 8) + 2 * w;
-                    const uint32_t key = pair[u * 8], v0 = pair[at], v1 = pair[at + 1];
+                    const int at = u * 16 / N + (N == 2 ? 0 : c / 2 * 8) + 2 * w;
+                    const uint32_t v0 = pair[at], v1 = pair[at + 1];
                     const uint32_t p0 = values ? v0 : key, p1 = values ? v1 : key;
-                    y[w] = bf16_pair(fmaf(bf16_lo(p0), bf16_lo(n[w]) - 128.0f, bf16_hi(p0)),
-                                     fmaf(bf16_lo(p1), bf16_hi(n[w]) - 128.0f, bf16_hi(p1)));
+                    const uint32_t from = w % 2 ? odd : even;
+                    const float c0 = (float)(from >> (w < 2 ? 0 : 8) & 0xFFu), c1 = (float)(from >> (w < 2 ? 16 : 24) & 0xFFu);
+                    y[w] = bf16_pair(fmaf(bf16_lo(p0), c0, bf16_hi(p0)), fmaf(bf16_lo(p1), c1, bf16_hi(p1)));
                 }
                 if (tail && values)
-                    y = keep_seen(y, (blk ? held1 : held0) >> (4 * (lane >> 5) + 16 * (U == 2 ? i : c / 2)), 0);
+                    y = keep_seen(y, (blk ? held1 : held0) >> (4 * (lane >> 5) + 16 * (N == 2 ? i : c / 2)), 0);
                 dst[(i * 4 + c) * 64 + lane] = y;
             }
         }
     }
 };
 
+// The work of a sequence in steps, and how its items follow each other.  Under a causal mask tile t takes about as many
+// steps more than the first as tile T - 1 - t takes fewer than the last: the two together are given a fixed number of
+// places, `pair`, at least what any such two need, so a place in the list is found without summing over tiles.  Order:
+// (head, pair of tiles, the shorter, the longer), the tile in the middle of an odd number alone at the end; a few places
+// at the end of each pair are empty.
+struct TileList {
+    uint32_t tiles, pair, middle, head;  // head: places of one head
+};
+
+__device__ __forceinline__ uint32_t steps_of(const AttendArgs &a, const SeqInfo &s, uint32_t tile) {
+    const uint32_t r0 = tile * kTileRows, r1 = min(r0 + kTileRows, rows_of(a, s));
+    return max((span_of(a, s, r0, r1).nb + 1) / 2, 1u);
+}
+
+__device__ __forceinline__ TileList tiles_in(const AttendArgs &a, const SeqInfo &s) {
+    TileList l;
+    l.tiles = (rows_of(a, s) + kTileRows - 1) / kTileRows;
+    if (l.tiles == 0) return TileList{0, 0, 0, 0};
+    // without a window a tile whose last row stands at p takes p / 64 + 1 steps; positions grow evenly from tile to tile (the
+    // last tile counted as a full one), rounded down, so two opposite tiles' sum at most 1 above the outer two's
+    const int32_t first = s.len - s.n;
+    const int32_t x = max(first + (int32_t)token_of(a, kTileRows - 1), 0);
+    const int32_t y = max(first + (int32_t)token_of(a, l.tiles * kTileRows - 1), 0);
+    l.pair = (uint32_t)(x + y + 1) / 64 + 2;
+    if (a.window) {  // a tile's blocks: the sinks', and those from its first row's window to its last row
+        const uint32_t tokens = token_of(a, kTileRows + a.group - 2) + 1;
+        const uint32_t blocks = ((uint32_t)a.sinks + kKvBlock - 1) / kKvBlock + ((uint32_t)a.window + tokens) / kKvBlock + 2;
+        l.pair = min(l.pair, 2 * ((blocks + 1) / 2));
+    }
+    l.middle = l.tiles % 2 ? steps_of(a, s, l.tiles / 2) : 0;
+    l.head = l.tiles / 2 * l.pair + l.middle;
+    return l;
+}
+
+// A tile's places: [begin, begin + places) of its head's.
+struct TilePlace {
+    uint32_t tile, begin, places;
+};
+__device__ __forceinline__ TilePlace tile_at(const AttendArgs &a, const SeqInfo &s, const TileList &l, uint32_t place) {
+    const uint32_t half = l.tiles / 2, k = l.pair ? min(place / l.pair, half) : 0;
+    if (k == half) return TilePlace{half, half * l.pair, l.middle};
+    const uint32_t shorter = steps_of(a, s, k), at = k * l.pair;
+    if (place - at < shorter) return TilePlace{k, at, shorter};
+    return TilePlace{l.tiles - 1 - k, at + shorter, l.pair - shorter};
+}
+// The list is cut every `share` places, but a cut near a tile's begin or end is moved there.  A cut tile's partial sums go
+// through memory, which costs about as much as eight steps (2 x 256 rows x D x 4 bytes written and read again, against
+// 256 x 64 x D x 4 flops a step), so a share may be that much uneven, or a sixteenth.
+struct RowShare {
+    uint32_t share, slack;
+    __device__ __forceinline__ RowShare(uint32_t total, uint32_t workers) {
+        share = max((total + workers - 1) / workers, kLeastShare);
+        slack = max(share / 16, 7u);
+    }
+    // where a cut `off` places behind a tile's begin (0 < off < places, or 0) goes
+    __device__ __forceinline__ uint32_t cut(uint32_t off, uint32_t places) const {
+        return off <= slack ? 0 : places - off <= slack ? places : off;
+    }
+};
+
+// Steps [u0, u1) of one tile of one head.
 template <int KIND, int D>
-__global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    uint32_t *word = reinterpret_cast<uint32_t *>(lds);
-    // Workgroups go to the eight XCDs in turn, and each has an L2 of its own: an XCD takes a contiguous run of the items in
-    // the order (sequence, head, tile), so that the tiles of a head read its keys and values through one L2.
-    Found f;
-    const auto items = [&](uint32_t i) {
-        bool x;
-        return (rows_of(a, load_seq(a.batch, a.cache, i, x)) + kTileRows - 1) / kTileRows * a.cache.kv_heads;
-    };
-    const auto mine = [&](uint32_t total) {
-        const uint32_t run = (total + 7) / 8, k = blockIdx.x >> 3;
-        return k < run ? (blockIdx.x & 7) * run + k : 0xFFFFFFFFu;
-    };
-    if (!locate(a.batch.seqs, items, mine, word, f)) return;
-    bool bad;
-    const SeqInfo s = load_seq(a.batch, a.cache, f.seq, bad);
-    if (bad && threadIdx.x == 0) report_bad_index(a.batch);
-    const uint32_t all_rows = rows_of(a, s), tiles = (all_rows + kTileRows - 1) / kTileRows;
-    const uint32_t head = (f.target - f.begin) / tiles, tile = tiles - 1 - (f.target - f.begin) % tiles;  // (longest first)
+__device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t seq, const SeqInfo &s, uint32_t head, uint32_t tile,
+                                                  uint32_t u0, uint32_t u1, bool whole, float *slot, uint8_t *lds) {
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-    const uint32_t t0 = tile * kTileRows, t1 = min(t0 + kTileRows, all_rows);
+    const uint32_t t0 = tile * kTileRows, t1 = min(t0 + kTileRows, rows_of(a, s));
     const Span span = span_of(a, s, t0, t1);
     const uint32_t r0 = t0 + wave * 32, r1 = min(r0 + 32, t1);
     const bool any = r0 < r1;
-    Span own = any ? span_of(a, s, r0, r1) : span;
+    const Span own = any ? span_of(a, s, r0, r1) : span;
     const Queries<D> q = load_queries<D>(a, s, head, r0 + col, t1);
-    const int32_t pos = s.len - s.n + (int32_t)((r0 + col) / a.group);
+    const int32_t pos = s.len - s.n + (int32_t)token_of(a, r0 + col);
     Running<D> run;
     run.clear();
 
+    const uint32_t last = min(u1, (span.nb + 1) / 2);
     const auto place = [&](uint32_t i, bool &gone) -> const uint8_t * {
         const uint32_t blk = span.block(min(i, span.nb - 1));
-        const uint32_t page = page_of(a.batch, a.cache, f.seq, blk);
+        const uint32_t page = uniform(page_of(a.batch, a.cache, seq, blk));
         gone = page == kNoPage;
         return block_at<KIND, D>(a.cache, gone ? 0 : page, head, blk);
     };
     Stage<KIND, D> stage;
     bool gone[2] = {false, false}, lost = false;
-    const uint32_t steps = (span.nb + 1) / 2;
-    if (steps) {
-        const uint8_t *b0 = place(0, gone[0]), *b1 = place(1, gone[1]);
+    if (u0 < last) {
+        const uint8_t *b0 = place(2 * u0, gone[0]), *b1 = place(2 * u0 + 1, gone[1]);
         stage.fetch(b0, b1);
     }
     const auto held = [&](int32_t kb, bool g) { return g ? 0u : bits(0, s.len - kb); };
-    for (uint32_t st = 0; st < steps; ++st) {
+    __syncthreads();  // (the LDS is free of the piece before)
+    for (uint32_t st = u0; st < last; ++st) {
         uint8_t *buf = lds + (st & 1) * (256 * D);
         const bool g0 = gone[0], g1 = gone[1] || 2 * st + 1 >= span.nb;
         const int32_t kb0 = (int32_t)(span.block(2 * st) * kKvBlock);
@@ -760,7 +818,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         stage.store(buf, held(kb0, g0), held(kb1, g1));
         lost = lost || g0 || gone[1];
         __syncthreads();
-        if (st + 1 < steps) {
+        if (st + 1 < last) {
             const uint8_t *b0 = place(2 * st + 2, gone[0]), *b1 = place(2 * st + 3, gone[1]);
             stage.fetch(b0, b1);
         }
@@ -807,9 +865,25 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
                 run.o[db] = mfma(kv[(s2 / 2) * kBlk + 4 * D + ((s2 % 2) * (D / 32) + db) * 64 + lane], p[s2], run.o[db]);
     }
     if (lost && threadIdx.x == 0) report_bad_index(a.batch);
-    const float l = run.l + other_half(run.l), inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float l = run.l + other_half(run.l);
     if (r0 + col >= t1) return;
-    const uint32_t tok = (r0 + col) / a.group, gh = head * a.group + (r0 + col) % a.group;
+    if (!whole) {
+        float *o = slot + (r0 - t0 + col) * D;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f32x4_p w = {run.o[db][4 * k], run.o[db][4 * k + 1], run.o[db][4 * k + 2], run.o[db][4 * k + 3]};
+                *reinterpret_cast<f32x4_p *>(o + 32 * db + 8 * k + 4 * h) = w;
+            }
+        if (h == 0) {
+            slot[kTileRows * D + r0 - t0 + col] = run.m;
+            slot[kTileRows * (D + 1) + r0 - t0 + col] = l;
+        }
+        return;
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const uint32_t tok = token_of(a, r0 + col), gh = head * a.group + r0 + col - tok * a.group;
     uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
@@ -821,6 +895,102 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(AttendArgs a) {
         }
     if (a.lse && h == 0)
         a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = run.m == kNone ? kNone : (run.m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int KIND, int D>
+__global__ __launch_bounds__(kRowThreads, D == 128 ? 2 : 4) void attend_rows_kernel(AttendArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint32_t *word = reinterpret_cast<uint32_t *>(lds);
+    // Workgroups go to the eight XCDs in turn, and each has an L2 of its own: an XCD takes a contiguous run of the list, so
+    // that the tiles of a head read its keys and values through one L2.
+    const uint32_t worker = (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
+    Found f;
+    const auto weight = [&](uint32_t i) {
+        bool x;
+        return tiles_in(a, load_seq(a.batch, a.cache, i, x)).head * a.cache.kv_heads;
+    };
+    if (!locate(a.batch.seqs, weight, [&](uint32_t total) { return worker * RowShare(total, gridDim.x).share; }, word, f)) return;
+    const RowShare cuts(f.total, gridDim.x);
+    uint32_t seq = f.seq, base = f.begin;  // of the list, where the sequence begins
+    const uint32_t end = min(f.target + cuts.share, f.total);
+    bool bad;
+    SeqInfo s = load_seq(a.batch, a.cache, seq, bad);
+    TileList list = tiles_in(a, s);
+    uint32_t place = f.target - base;
+    bool begins = true;  // the first tile: the cut before this workgroup
+    for (;;) {
+        if (bad && threadIdx.x == 0) report_bad_index(a.batch);
+        const uint32_t head = place / list.head;
+        const TilePlace t = tile_at(a, s, list, place - head * list.head);
+        const uint32_t at = base + head * list.head + t.begin;  // where the tile begins in the list
+        if (at >= end) return;
+        const uint32_t u0 = begins ? cuts.cut(f.target - at, t.places) : 0;
+        const uint32_t u1 = end - at >= t.places ? t.places : cuts.cut(end - at, t.places);
+        begins = false;
+        if (u0 < u1) {
+            // a tile that goes on from the workgroup before leaves its sums in slot 0, one that goes on in the next in slot 1
+            float *slot = a.work + (uint64_t)(worker * 2 + (u0 == 0 ? 1 : 0)) * (kTileRows * (D + 2));
+            attend_rows_piece<KIND, D>(a, seq, s, head, t.tile, u0, u1, u0 == 0 && u1 == t.places, slot, lds);
+        }
+        place = head * list.head + t.begin + t.places;
+        if (place < list.head * a.cache.kv_heads) continue;
+        base += place;
+        place = 0;
+        do {
+            if (++seq >= a.batch.seqs) return;
+            s = load_seq(a.batch, a.cache, seq, bad);
+            list = tiles_in(a, s);
+        } while (list.head == 0);
+    }
+}
+
+// 32 rows of the tile that the cut before workgroup blockIdx.x + 1 goes through: the sum of its parts.
+template <int D>
+__global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uint32_t workers) {
+    __shared__ uint32_t word[10];
+    const uint32_t k = blockIdx.x + 1;
+    Found f;
+    const auto weight = [&](uint32_t i) {
+        bool x;
+        return tiles_in(a, load_seq(a.batch, a.cache, i, x)).head * a.cache.kv_heads;
+    };
+    if (!locate(a.batch.seqs, weight, [&](uint32_t total) { return k * RowShare(total, workers).share; }, word, f)) return;
+    const RowShare cuts(f.total, workers);
+    bool bad;
+    const SeqInfo s = load_seq(a.batch, a.cache, f.seq, bad);
+    const TileList list = tiles_in(a, s);
+    const uint32_t place = f.target - f.begin, head = place / list.head;
+    const TilePlace t = tile_at(a, s, list, place - head * list.head);
+    const uint32_t at = f.begin + head * list.head + t.begin, off = f.target - at;
+    const uint32_t moved = cuts.cut(off, t.places);
+    if (moved == 0 || moved == t.places) return;                                      // not cut here
+    if (off > cuts.share && cuts.cut(off - cuts.share, t.places) != 0) return;  // cut before: joined there
+    const uint32_t t0 = t.tile * kTileRows, r0 = t0 + blockIdx.y * 32, r1 = min(r0 + 32, rows_of(a, s));
+    const uint32_t w0 = k - 1;
+    uint32_t w1 = (at + t.places - 1) / cuts.share;
+    if (w1 > k && cuts.cut(w1 * cuts.share - at, t.places) == t.places) --w1;
+    constexpr uint32_t kLanes = D / 4;
+    const uint32_t d = threadIdx.x % kLanes * 4;
+    for (uint32_t r = r0 + threadIdx.x / kLanes; r < r1; r += 256 / kLanes) {
+        float m = kNone, l = 0.0f;
+        f32x4_p acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t w = w0; w <= w1; ++w) {
+            const float *slot = a.work + (uint64_t)(w * 2 + (w == w0 ? 1 : 0)) * (kTileRows * (D + 2));
+            const float mw = slot[kTileRows * D + r - t0], lw = slot[kTileRows * (D + 1) + r - t0];
+            const f32x4_p y = *reinterpret_cast<const f32x4_p *>(slot + (r - t0) * D + d);
+            const float top = fmaxf(m, mw), f0 = m == kNone ? 0.0f : exp2_fast(m - top), f1 = mw == kNone ? 0.0f : exp2_fast(mw - top);
+            l = l * f0 + lw * f1;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f0 + y[c] * f1;
+            m = top;
+        }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const uint32_t tok = token_of(a, r), gh = head * a.group + r - tok * a.group;
+        u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+        *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
+        if (a.lse && d == 0)
+            a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -838,7 +1008,7 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t head_dim, uin
     if (int rc = cu_count(&cus)) return rc;
     const uint64_t rows = (uint64_t)b.tokens * group;
     const uint64_t per_seq = (uint64_t)(b.start ? new_longest : 1) * group;
-    p->many = per_seq >= 64 && rows * v.kv_heads / kTileRows >= cus / 2;
+    p->many = per_seq >= 64 && rows * v.kv_heads / kTileRows >= cus / 4;
     p->whole = false;
     p->work_bytes = 0;
     p->rp = per_seq <= 4 ? 4 : per_seq <= 8 ? 8 : per_seq <= 16 ? 16 : 32;
@@ -847,7 +1017,9 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t head_dim, uin
     if (items > 0x7FFFFF00ull) return fail(CI_ERR_ARG, "ci_paged_attention: too many rows for one call");
     p->items = (uint32_t)items;
     if (p->many) {
-        p->grid = (p->items + 7) / 8 * 8;
+        // as many as are resident: two wavefronts per SIMD for heads of 128, four for heads of 64
+        p->workers = p->grid = ((head_dim == 128 ? 512 : 1024) * cus / kRowThreads + 7) / 8 * 8;
+        p->work_bytes = (size_t)p->workers * 2 * kTileRows * (head_dim + 2) * sizeof(float);
         return CI_OK;
     }
     uint64_t keys = longest;
@@ -875,8 +1047,12 @@ template <int KIND, int D>
 static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
     if (p.many) {
         CI_ALLOW_FULL_LDS((attend_rows_kernel<KIND, D>));
-        CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(256), rows_lds(D), s, a);
+        CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(kRowThreads), rows_lds(D), s, a);
         CI_LAUNCH_CHECK("attend_rows_kernel");
+        if (p.workers > 1) {
+            CI_KV_LAUNCH((attend_rows_join_kernel<D>), dim3(p.workers - 1, kTileRows / 32), dim3(256), 0, s, a, p.workers);
+            CI_LAUNCH_CHECK("attend_rows_join_kernel");
+        }
         return CI_OK;
     }
     switch (p.rp) {
@@ -938,6 +1114,7 @@ extern "C" int ci_paged_attention(const ci_kv_cache *cache, const ci_kv_batch *b
     a.l_row = lse_stride;
     a.q_row = q->row_stride, a.q_head = q->head_stride, a.o_row = out->row_stride, a.o_head = out->head_stride;
     a.group = q_heads / a.cache.kv_heads;
+    a.per_group = 1.0 / (double)a.group;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.window = window < (1 << 30) ? window : 1 << 30;  // (no sequence is longer: sums of positions stay in 32 bits)
     a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;

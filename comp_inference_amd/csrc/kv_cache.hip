@@ -185,7 +185,7 @@ __device__ __forceinline__ uint32_t row_pair(u32x4 a, u32x4 b) {
 
 template <int KIND, int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs p) {
-    __shared__ uint32_t word[8];
+    __shared__ uint32_t word[10];
     __shared__ uint32_t codes[256 / (D / 16) * D / 8];  // 4 bits: the values' codes of the rows in hand
     constexpr uint32_t kSlots = D / 16, kRows = 256 / kSlots;
     const Tile t = find_tile(p.batch, p.cache, blockIdx.x, word);
@@ -310,7 +310,7 @@ struct ReadArgs {
 // (rounded once to 32 bits, then to bf16).
 template <int KIND, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs p) {
-    __shared__ uint32_t word[8];
+    __shared__ uint32_t word[10];
     constexpr uint32_t kSlots = D / 8;
     const Tile t = find_tile(p.batch, p.cache, blockIdx.x, word);
     if (t.bad && threadIdx.x == 0 && blockIdx.y == 0) report_bad_index(p.batch);

@@ -117,8 +117,9 @@ __device__ __forceinline__ uint8_t *block_at(const KvView &v, uint32_t page, uin
     return v.data + index * KvBlock<KIND, D>::kBytes;
 }
 
-// Exclusive prefix sum over the 256 threads of a workgroup; `total` gets the sum.  `part` holds four words of LDS.
-__device__ __forceinline__ uint32_t scan256(uint32_t x, uint32_t *part, uint32_t &total) {
+// Exclusive prefix sum over the threads of a workgroup (up to eight wavefronts); `total` gets the sum.  `part` holds eight
+// words of LDS.
+__device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t *part, uint32_t &total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t inc = x;
 #pragma unroll
@@ -131,8 +132,7 @@ __device__ __forceinline__ uint32_t scan256(uint32_t x, uint32_t *part, uint32_t
     __syncthreads();
     uint32_t before = 0;
     total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < 4; ++w) {
+    for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
         const uint32_t p = part[w];
         if (w < wave) before += p;
         total += p;
@@ -142,17 +142,17 @@ __device__ __forceinline__ uint32_t scan256(uint32_t x, uint32_t *part, uint32_t
 
 // A running sum over the sequences, weight(i) each (evaluated by one thread: a contiguous run of sequences per thread).
 // `target` maps the total to the place looked for: the sequence in whose share it falls, and where that share begins.
-// Returns false when there is no such place.  `word` holds eight words of LDS.
+// Returns false when there is no such place.  `word` holds ten words of LDS.
 struct Found {
     uint32_t seq, begin, total, target;
 };
 
 template <typename W, typename T>
 __device__ __forceinline__ bool locate(uint32_t seqs, W weight, T target, uint32_t *word, Found &f) {
-    const uint32_t per = (seqs + 255) / 256, first = min(threadIdx.x * per, seqs), last = min(first + per, seqs);
+    const uint32_t per = (seqs + blockDim.x - 1) / blockDim.x, first = min(threadIdx.x * per, seqs), last = min(first + per, seqs);
     uint32_t mine = 0;
     for (uint32_t i = first; i < last; ++i) mine += weight(i);
-    uint32_t at = scan256(mine, word, f.total);
+    uint32_t at = scan_threads(mine, word, f.total);
     f.total = (uint32_t)__builtin_amdgcn_readfirstlane((int)f.total);
     f.target = target(f.total);
     if (f.target >= f.total) return false;
@@ -163,12 +163,12 @@ __device__ __forceinline__ bool locate(uint32_t seqs, W weight, T target, uint32
             if (f.target - at < w) break;
             at += w;
         }
-        word[4] = i;
-        word[5] = at;
+        word[8] = i;
+        word[9] = at;
     }
     __syncthreads();
-    f.seq = (uint32_t)__builtin_amdgcn_readfirstlane((int)word[4]);
-    f.begin = (uint32_t)__builtin_amdgcn_readfirstlane((int)word[5]);
+    f.seq = (uint32_t)__builtin_amdgcn_readfirstlane((int)word[8]);
+    f.begin = (uint32_t)__builtin_amdgcn_readfirstlane((int)word[9]);
     __syncthreads();
     return true;
 }
