@@ -147,6 +147,91 @@ __device__ __forceinline__ Queries<D> load_queries(const AttendArgs &a, const Se
     return q;
 }
 
+// ---- one row, the plain way -----------------------------------------------------------------------------------------
+// A wavefront goes over the keys of one row, 64 at a time, and adds up only what the row sees.  In the kernels below a
+// matrix instruction multiplies the values of keys that SOME row of its tile sees by weights that are zero for the others;
+// where such a value is an infinity or a NaN, and where a page was none of the cache's (its keys are unseen), the row's
+// result comes out as no number, and the row is done again here.  Slow, and right.
+template <int KIND, int D>
+__device__ __forceinline__ void attend_one_row(const AttendArgs &a, uint32_t seq, const SeqInfo &s, uint32_t head, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63, tok = token_of(a, row), gh = head * a.group + row - tok * a.group;
+    const int32_t p = s.len - s.n + (int32_t)tok;
+    const uint16_t *q = a.q + (int64_t)(s.row + (int32_t)tok) * a.q_row + (int64_t)gh * a.q_head;
+    float m = kNone, l = 0.0f, o[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[i] = 0.0f;
+#pragma unroll 1
+    for (int32_t base = 0; base <= p; base += 64) {
+        const int32_t j = base + (int32_t)lane;
+        bool seen = j <= p && (!a.window || p - j < a.window || j < a.sinks);
+        if (!__builtin_amdgcn_ballot_w64(seen)) continue;
+        const uint32_t page = seen ? page_of(a.batch, a.cache, seq, (uint32_t)j / kKvBlock) : kNoPage;
+        seen = page != kNoPage;
+        const uint64_t who = __builtin_amdgcn_ballot_w64(seen);
+        if (!who) continue;
+        const uint8_t *block = block_at<KIND, D>(a.cache, seen ? page : 0, head, (uint32_t)j / kKvBlock);
+        const uint32_t t = (uint32_t)j % kKvBlock;
+        float x = 0.0f;
+        const uint32_t *pairs = reinterpret_cast<const uint32_t *>(block + KvBlock<KIND, D>::kPairs);
+        const uint32_t kp = KIND == CI_KV_BF16 ? 0 : pairs[t];
+#pragma unroll 1
+        for (uint32_t c = 0; c < D / 8; ++c) {
+            const u32x4 y = *reinterpret_cast<const u32x4 *>(q + 8 * c);
+            u32x4 k{};
+            uint32_t word = 0;
+            if (KIND == CI_KV_BF16)
+                k = reinterpret_cast<const u32x4 *>(block)[key_operand(c, t)];
+            else
+                word = reinterpret_cast<const uint32_t *>(block)[key_word(c, t)];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                const float ye = e & 1 ? bf16_hi(y[e / 2]) : bf16_lo(y[e / 2]);
+                const float ke = KIND != CI_KV_BF16 ? fmaf((float)(word >> nibble_shift(e) & 15u), bf16_lo(kp), bf16_hi(kp))
+                                 : e & 1            ? bf16_hi(k[e / 2])
+                                                    : bf16_lo(k[e / 2]);
+                x = fmaf(ye, ke, x);
+            }
+        }
+        x = seen ? x * a.scale_log2 : kNone;
+        float top = most(m, x);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) top = most(top, lane_xor(top, d));
+        const float f = m == kNone ? 0.0f : exp2_fast(m - top);
+        float w = seen && top != kNone ? exp2_fast(x - top) : 0.0f, sum = w;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) sum += lane_xor(sum, d);
+        l = l * f + sum;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) o[i] *= f;
+        m = top;
+#pragma unroll 1
+        for (uint32_t k = 0; k < 64; ++k) {
+            if (!(who >> k & 1)) continue;
+            const float wk = __int_as_float(__shfl(__float_as_int(w), (int)k, 64));
+            const uint32_t pk = (uint32_t)__shfl((int)page, (int)k, 64), blk = (uint32_t)(base + (int32_t)k) / kKvBlock, tk = (uint32_t)(base + (int32_t)k) % kKvBlock;
+            const uint8_t *vals = block_at<KIND, D>(a.cache, pk, head, blk) + KvBlock<KIND, D>::kHalf;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const uint32_t at = value_operand<D>(lane + 64 * i, tk), e = value_element(tk);
+                float v;
+                if (KIND == CI_KV_BF16) {
+                    v = bf16_lo(reinterpret_cast<const uint16_t *>(vals)[at * 8 + e]);
+                } else {
+                    const uint32_t vp = reinterpret_cast<const uint32_t *>(vals - KvBlock<KIND, D>::kHalf + KvBlock<KIND, D>::kPairs)[kKvBlock + tk];
+                    v = fmaf((float)(reinterpret_cast<const uint32_t *>(vals)[value_word(at)] >> nibble_shift(e) & 15u), bf16_lo(vp), bf16_hi(vp));
+                }
+                o[i] += wk * v;
+            }
+        }
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (uint16_t)bf16_pair(o[i] * inv, 0.0f);
+    if (a.lse && lane == 0) a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
+}
+__device__ __forceinline__ bool no_number(float x) { return !(fabsf(x) < __builtin_inff()); }
+
 // ---- few rows -------------------------------------------------------------------------------------------------------
 // RP columns of the 32 are rows; the columns c, c + RP, c + 2 RP .. hold the same row.  Every one of them gets all 32 scores
 // of a block in the product, and works on 32 / RP of them only: column c + j RP takes elements [j NV, (j + 1) NV) of its
@@ -316,31 +401,30 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
 #pragma unroll
         for (int i = 0; i < Data::N; ++i) x.v[i] = reinterpret_cast<const u32x4 *>(b + KvBlock<KIND, D>::kHalf)[i * 64 + lane];
     };
-    // the block of a step; a page that is none of the cache's: some page, its keys unseen
-    auto place = [&](uint32_t i, bool &gone) -> const uint8_t * {
+    PageRun table(a.batch, it.seq);
+    // the block of a step (of a page that is none of the cache's: page 0; the item's rows are done again)
+    auto place = [&](uint32_t i) -> const uint8_t * {
         const uint32_t blk = span.block(i);
-        const uint32_t page = uniform(page_of(a.batch, a.cache, it.seq, blk));
-        gone = page == kNoPage;
-        return block_at<KIND, D>(a.cache, gone ? 0 : page, it.head, blk);
+        table.hold(a.batch, a.cache, blk);
+        const uint32_t page = table.page_of(a.cache, blk);
+        lost = lost || page == kNoPage;
+        return block_at<KIND, D>(a.cache, page == kNoPage ? 0 : page, it.head, blk);
     };
 
     // keys are asked for one step ahead, values at the head of their step: a wavefront always has half a block on its way
     Data x;
     uint32_t i = u0 * kUnit + wave;
     const uint8_t *b = nullptr;
-    bool gone_next = false;
     if (i < last) {
-        b = place(i, gone_next);
+        b = place(i);
         fetch_k(b, x);
     }
     for (; i < last; i += kUnit) {
         const int32_t kb = (int32_t)(span.block(i) * kKvBlock);
-        const bool gone = gone_next;
-        lost = lost || gone;
         fetch_v(b, x);
-        const bool edge = gone || !all_visible(a, span, kb);
+        const bool edge = !all_visible(a, span, kb);
         uint32_t sees = 0xFFFFFFFFu;  // the lane's keys that its row sees, key0 as bit 0
-        if (edge) sees = gone ? 0u : seen_keys(a, pos, pos, kb) >> cols.key0;
+        if (edge) sees = seen_keys(a, pos, pos, kb) >> cols.key0;
         f32x16_p acc = start;
         if (KIND == CI_KV_BF16) {
 #pragma unroll
@@ -355,7 +439,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             cols.pairs(pairs, kp);
             cols.pairs(pairs + kKvBlock, vp);
         }
-        b = place(min(i + kUnit, last - 1), gone_next);
+        b = place(min(i + kUnit, last - 1));
         fetch_k(b, x);
         float t[NV];
         cols.take(acc, t);
@@ -394,7 +478,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
         u32x4 f[2];
         cols.give(pk, f);
         if (KIND == CI_KV_BF16 && edge) {
-            const uint32_t seen = gone ? 0u : seen_keys(a, span.p_lo, span.p_hi, kb) >> (4 * h);
+            const uint32_t seen = seen_keys(a, span.p_lo, span.p_hi, kb) >> (4 * h);
 #pragma unroll
             for (int k = 0; k < Data::N; ++k) x.v[k] = keep_seen(x.v[k], seen, (uint32_t)k / (D / 32));
         }
@@ -406,11 +490,15 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
                 run.o[db] = mfma(KIND == CI_KV_BF16 ? x.v[k % Data::N] : codes_to_bf16(x.v[k / 4][k % 4]), f[s2], run.o[db]);
             }
     }
-    if (lost && lane == 0) report_bad_index(a.batch);
+    if (lost) {
+        if (lane == 0) report_bad_index(a.batch);
+        run.l = __builtin_nanf("");  // (the rows will be found to be no numbers, and done again)
+    }
 
     // ---- join: the columns of a wavefront that hold the same row (c, c + RP, ..), then the four wavefronts
     float *o_lds = reinterpret_cast<float *>(lds);                      // [4][32][kStride]
     float *m_lds = o_lds + 4 * 32 * kStride, *l_lds = m_lds + 4 * RP;  // [4][RP] each
+    uint32_t *again = reinterpret_cast<uint32_t *>(l_lds + 4 * RP);    // rows that are no numbers, a bit each
     run.l += other_half(run.l);
     run.off += other_half(run.off);
     float m = run.m;
@@ -421,6 +509,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
 #pragma unroll
     for (int d = RP; d < 32; d *= 2) l += lane_xor(l, d);
     __syncthreads();  // (the LDS is free of the piece before)
+    if (threadIdx.x == 0) *again = 0;
     if (lane < RP) {
         m_lds[wave * RP + lane] = m;
         l_lds[wave * RP + lane] = l;
@@ -455,6 +544,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing: zeros)
             const uint32_t tok = token_of(a, r0 + rr), g = r0 + rr - tok * a.group;
             u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+            if (no_number(acc[0] * inv + acc[1] * inv + (acc[2] * inv + acc[3] * inv))) atomicOr(again, 1u << rr);
             *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row +
                                        (int64_t)(it.head * a.group + g) * a.o_head + d) = w;
             if (a.lse && d == 0)
@@ -468,11 +558,16 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             }
         }
     }
+    if (whole) {
+        __syncthreads();
+        for (uint32_t rr = wave; rr < rows; rr += 4)
+            if (uniform(*again) >> rr & 1) attend_one_row<KIND, D>(a, it.seq, s, it.head, r0 + rr);
+    }
 }
 
 template <int D, int RP>
 constexpr uint32_t slot_floats() { return RP * (D + 2); }
-constexpr uint32_t split_lds(int D) { return (4 * 32 * (D + 4) + 2 * 4 * 32) * 4; }
+constexpr uint32_t split_lds(int D) { return (4 * 32 * (D + 4) + 2 * 4 * 32 + 4) * 4; }
 
 // Units of all items in the order (sequence, tile, head), cut evenly.
 __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t workers) { return max((total + workers - 1) / workers, 1u); }
@@ -531,7 +626,7 @@ __global__ __launch_bounds__(256, 2) void attend_split_kernel(AttendArgs a) {
 }
 
 // One row of one item that was cut: the sum of its parts, which 256 / (D / 4) groups of threads take in turn.
-template <int D, int RP>
+template <int KIND, int D, int RP>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t workers) {
     constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes;
     __shared__ uint32_t word[10];
@@ -599,35 +694,47 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
     }
     *reinterpret_cast<f32x4_p *>(part + threadIdx.x * 4) = acc;
     if (d == 0) part_l[g] = l, part_m[g] = m;
+    if (threadIdx.x == 0) word[0] = 0;
     __syncthreads();
-    if (threadIdx.x >= kLanes) return;
-    m = kNone;
+    if (threadIdx.x < kLanes) {
+        m = kNone;
 #pragma unroll
-    for (uint32_t k = 0; k < kGroups; ++k) m = fmaxf(m, part_m[k]);
-    l = 0.0f;
-    acc = f32x4_p{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t k = 0; k < kGroups; ++k) m = fmaxf(m, part_m[k]);
+        l = 0.0f;
+        acc = f32x4_p{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (uint32_t k = 0; k < kGroups; ++k) {
-        const float f = part_m[k] == kNone ? 0.0f : exp2_fast(part_m[k] - m);
-        l += f * part_l[k];
-        const f32x4_p y = *reinterpret_cast<const f32x4_p *>(part + (k * kLanes + threadIdx.x) * 4);
+        for (uint32_t k = 0; k < kGroups; ++k) {
+            const float f = part_m[k] == kNone ? 0.0f : exp2_fast(part_m[k] - m);
+            l += f * part_l[k];
+            const f32x4_p y = *reinterpret_cast<const f32x4_p *>(part + (k * kLanes + threadIdx.x) * 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
+            for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
+        }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const uint32_t tok = token_of(a, r0 + row), gh = it.head * a.group + r0 + row - tok * a.group;
+        u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
+        *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
+        if (a.lse && d == 0)
+            a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
+        if (no_number(acc[0] * inv + acc[1] * inv + (acc[2] * inv + acc[3] * inv))) atomicOr(word, 1u);
     }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const uint32_t tok = token_of(a, r0 + row), gh = it.head * a.group + r0 + row - tok * a.group;
-    u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
-    *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
-    if (a.lse && d == 0)
-        a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
+    __syncthreads();
+    if (threadIdx.x < 64 && uniform(word[0])) attend_one_row<KIND, D>(a, it.seq, s, it.head, r0 + row);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------
+constexpr uint32_t kStep = 64;  // keys
 constexpr uint32_t kRowWaves = 8, kRowThreads = 64 * kRowWaves, kTileRows = 32 * kRowWaves;
 constexpr uint32_t rows_lds(int D) { return 2 * 2 * 128 * D; }  // two buffers of two blocks, keys and values in bf16
+// Workgroups resident on a CU: registers allow two wavefronts per SIMD, four for heads of 64 in bf16.
+constexpr uint32_t row_groups(uint32_t kind, uint32_t dim) { return kind == CI_KV_BF16 && dim == 64 ? 2 : 1; }
 constexpr uint32_t kLeastShare = 16;                             // steps (of 64 keys) worth a workgroup
 
-// What a thread carries of the next step from memory to the LDS.
+struct Blocks {  // the two blocks of a step
+    const uint8_t *b0, *b1;
+};
+
+// What a thread carries from memory to the LDS: its part of the keys of one step and of the values of the step before.
 template <int KIND, int D>
 struct Stage;
 
@@ -639,84 +746,99 @@ template <int D>
 struct Stage<CI_KV_BF16, D> {
     static constexpr int N = 256 * D / (16 * kRowThreads);  // 16-byte pieces per thread of two blocks of 128 D bytes
     u32x4 x[N];
-    static __device__ __forceinline__ uint32_t piece(int i) { return i * kRowThreads + threadIdx.x; }
-    __device__ __forceinline__ void fetch(const uint8_t *b0, const uint8_t *b1) {
+    static __device__ __forceinline__ uint32_t piece(int i) { return (i % (N / 2)) * kRowThreads + threadIdx.x; }  // of its block
+    static __device__ __forceinline__ bool is_value(int i) { return uniform(piece(i)) >= 4 * D; }
+    __device__ __forceinline__ void fetch(const Blocks &k, const Blocks &v) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint8_t *k01 = i < N / 2 ? k.b0 : k.b1, *v01 = i < N / 2 ? v.b0 : v.b1;
+            x[i] = reinterpret_cast<const u32x4 *>(is_value(i) ? v01 : k01)[piece(i)];
+        }
+    }
+    // values of tokens that are not there become zero
+    __device__ __forceinline__ void clear(uint32_t held0, uint32_t held1) {
+        const uint32_t h = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            x[i] = reinterpret_cast<const u32x4 *>(i < N / 2 ? b0 : b1)[piece(i % (N / 2))];
+            if (is_value(i)) x[i] = keep_seen(x[i], (i < N / 2 ? held0 : held1) >> (16 * ((piece(i) - 4 * D) / (2 * D)) + 4 * h), 0);
     }
-    __device__ __forceinline__ void store(uint8_t *lds, uint32_t held0, uint32_t held1) {
-        if ((held0 & held1) != 0xFFFFFFFFu) {
-            const uint32_t h = (threadIdx.x >> 5) & 1;
+    __device__ __forceinline__ void convert() {}
+    // keys to buffer `kb`, values to buffer `vb`
+    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb) const {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const uint32_t at = piece(i % (N / 2)), held = i < N / 2 ? held0 : held1;
-                if (at < 4 * D) continue;  // (keys)
-                x[i] = keep_seen(x[i], held >> (16 * ((at - 4 * D) / (2 * D)) + 4 * h), 0);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) reinterpret_cast<u32x4 *>(lds)[piece(i)] = x[i];
+        for (int i = 0; i < N; ++i)
+            reinterpret_cast<u32x4 *>((is_value(i) ? vb : kb) + (i < N / 2 ? 0 : 128 * D))[piece(i)] = x[i];
     }
 };
 
 // 4 bits: the codes become the values they stand for, rounded to bf16 (what a bf16 cache would hold of them), once for the
-// wavefronts that use them.  A wavefront takes whole 1 KB pieces of codes, keys or values of one block.
+// wavefronts that use them.  A wavefront takes a whole 1 KB piece of codes, keys or values of one block (for heads of 64
+// there are four pieces, and the second group has none).
 template <int D>
 struct Stage<CI_KV_INT4, D> {
-    static constexpr int N = D / 64;                                      // pieces of the keys of a block
-    static constexpr int U = 4 * N > (int)kRowWaves ? 4 * N / kRowWaves : 1;  // pieces per wavefront
-    u32x4 x[U];
-    uint32_t pair[U * 16 / N];  // (step, low): of the lane's key, or of its tokens (16 for heads of 64, 8 for 128)
-    static __device__ __forceinline__ uint32_t unit(int u) { return uniform(threadIdx.x >> 6) + kRowWaves * u; }
-    __device__ __forceinline__ void fetch(const uint8_t *b0, const uint8_t *b1) {
+    static constexpr int N = D / 64;  // pieces of the keys of a block
+    u32x4 x, y[4];
+    uint32_t own, pair[16 / N];  // (step, low): of the lane's key; of its tokens in the values (16 for heads of 64, 8 for 128)
+    uint32_t held = 0xFFFFFFFFu;  // tokens of the piece's block that are there
+    static __device__ __forceinline__ uint32_t unit() { return uniform(threadIdx.x >> 6); }
+    static __device__ __forceinline__ bool idle() { return unit() >= 4 * N; }
+    static __device__ __forceinline__ uint32_t block() { return unit() / (2 * N) & 1; }
+    static __device__ __forceinline__ uint32_t values() { return unit() / N & 1; }
+    static __device__ __forceinline__ uint32_t index() { return unit() % N; }
+    __device__ __forceinline__ void fetch(const Blocks &kb, const Blocks &vb) {
         const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
+        // (chosen by arithmetic: a choice between the four would put them into memory)
+        const int64_t blk = -(int64_t)block(), val = -(int64_t)values();
+        const uint8_t *k = kb.b0 + ((kb.b1 - kb.b0) & blk), *v = vb.b0 + ((vb.b1 - vb.b0) & blk), *b = k + ((v - k) & val);
+        x = reinterpret_cast<const u32x4 *>(b + values() * KvBlock<CI_KV_INT4, D>::kHalf)[index() * 64 + lane];
+        // tokens 16 s + 8 a + 4 h + b, s = the piece's index for heads of 128
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(b + KvBlock<CI_KV_INT4, D>::kPairs);
+        own = p[lane & 31];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (unit(u) >= 4 * N) continue;
-            const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
-            const uint8_t *b = blk ? b1 : b0;
-            x[u] = reinterpret_cast<const u32x4 *>(b + values * KvBlock<CI_KV_INT4, D>::kHalf)[i * 64 + lane];
-            const uint32_t *p = reinterpret_cast<const uint32_t *>(b + KvBlock<CI_KV_INT4, D>::kPairs);
-            const uint32_t key = p[lane & 31];
+        for (uint32_t c = 0; c < 16 / N; c += 4) {
+            const uint32_t s = N == 2 ? index() : c / 8;
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(p + kKvBlock + 16 * s + 8 * (c / 4 % 2) + 4 * h);
 #pragma unroll
-            for (int c = 0; c < 16 / N; c += 4) {  // tokens 16 s + 8 a + 4 h + b, s = i for heads of 128
-                const uint32_t s = N == 2 ? i : c / 8;
-                const u32x4 w = *reinterpret_cast<const u32x4 *>(p + kKvBlock + 16 * s + 8 * (c / 4 % 2) + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pair[u * 16 / N + c + e] = w[e];
-            }
-            if (!values) pair[u * 16 / N] = key;
+            for (int e = 0; e < 4; ++e) pair[c + e] = w[e];
         }
     }
-    __device__ __forceinline__ void store(uint8_t *lds, uint32_t held0, uint32_t held1) const {
+    __device__ __forceinline__ void clear(uint32_t held0, uint32_t held1) { held = block() ? held1 : held0; }
+    __device__ __forceinline__ void convert() {
+        if (idle()) return;
         const uint32_t lane = threadIdx.x & 63;
-        const bool tail = (held0 & held1) != 0xFFFFFFFFu;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (unit(u) >= 4 * N) continue;
-            const uint32_t blk = unit(u) / (2 * N), values = unit(u) / N % 2, i = unit(u) % N;
-            u32x4 *dst = reinterpret_cast<u32x4 *>(lds + blk * 128 * D + values * 64 * D);
-            const uint32_t key = pair[u * 16 / N];
+        if (values()) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                // codes 0, 4, 1, 5 and 2, 6, 3, 7 of the operand, a byte each
-                const uint32_t even = x[u][c] & 0x0F0F0F0Fu, odd = x[u][c] >> 4 & 0x0F0F0F0Fu;
-                u32x4 y;
+                float step[8], low[8];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int at = u * 16 / N + (N == 2 ? 0 : c / 2 * 8) + 2 * w;
-                    const uint32_t v0 = pair[at], v1 = pair[at + 1];
-                    const uint32_t p0 = values ? v0 : key, p1 = values ? v1 : key;
-                    const uint32_t from = w % 2 ? odd : even;
-                    const float c0 = (float)(from >> (w < 2 ? 0 : 8) & 0xFFu), c1 = (float)(from >> (w < 2 ? 16 : 24) & 0xFFu);
-                    y[w] = bf16_pair(fmaf(bf16_lo(p0), c0, bf16_hi(p0)), fmaf(bf16_lo(p1), c1, bf16_hi(p1)));
-                }
-                if (tail && values)
-                    y = keep_seen(y, (blk ? held1 : held0) >> (4 * (lane >> 5) + 16 * (N == 2 ? i : c / 2)), 0);
-                dst[(i * 4 + c) * 64 + lane] = y;
+                for (int e = 0; e < 8; ++e) step[e] = bf16_lo(pair[(N == 2 ? 0 : c / 2 * 8) + e]), low[e] = bf16_hi(pair[(N == 2 ? 0 : c / 2 * 8) + e]);
+                y[c] = eight(x[c], step, low);
+                if (held != 0xFFFFFFFFu) y[c] = keep_seen(y[c], held >> (4 * (lane >> 5) + 16 * (N == 2 ? index() : c / 2)), 0);
             }
+        } else {
+            float step[8], low[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) step[e] = bf16_lo(own), low[e] = bf16_hi(own);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = eight(x[c], step, low);
         }
+    }
+    static __device__ __forceinline__ u32x4 eight(uint32_t word, const float (&step)[8], const float (&low)[8]) {
+        const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;  // codes 0, 4, 1, 5 and 2, 6, 3, 7, a byte each
+        u32x4 r;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t from = w % 2 ? odd : even;
+            const float c0 = (float)(from >> (w < 2 ? 0 : 8) & 0xFFu), c1 = (float)(from >> (w < 2 ? 16 : 24) & 0xFFu);
+            r[w] = bf16_pair(fmaf(step[2 * w], c0, low[2 * w]), fmaf(step[2 * w + 1], c1, low[2 * w + 1]));
+        }
+        return r;
+    }
+    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb) const {
+        if (idle()) return;
+        u32x4 *dst = reinterpret_cast<u32x4 *>((values() ? vb : kb) + block() * 128 * D + values() * 64 * D) + index() * 256 + (threadIdx.x & 63);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) dst[c * 64] = y[c];
     }
 };
 
@@ -729,9 +851,28 @@ struct TileList {
     uint32_t tiles, pair, middle, head;  // head: places of one head
 };
 
+// The steps (64 keys from a multiple of 64) that rows at p_lo .. p_hi see a key of: [0, s1) and [w0, w0 + n - s1).
+struct Steps {
+    uint32_t s1, w0, n;
+    __device__ __forceinline__ int32_t first_key(uint32_t i) const { return (int32_t)((i < s1 ? i : i - s1 + w0) * kStep); }
+};
+__device__ __forceinline__ Steps steps_between(const AttendArgs &a, int32_t p_lo, int32_t p_hi) {
+    Steps x{};
+    const uint32_t end = p_hi < 0 ? 0 : (uint32_t)p_hi / kStep + 1;
+    if (a.window) {
+        x.w0 = p_lo - a.window + 1 > 0 ? (uint32_t)(p_lo - a.window + 1) / kStep : 0;
+        x.s1 = min(((uint32_t)a.sinks + kStep - 1) / kStep, end);
+        if (x.s1 >= x.w0) x.s1 = x.w0 = 0;
+    }
+    x.n = x.s1 + end - x.w0;
+    return x;
+}
+__device__ __forceinline__ int32_t position_of(const AttendArgs &a, const SeqInfo &s, uint32_t row) {
+    return s.len - s.n + (int32_t)token_of(a, row);
+}
 __device__ __forceinline__ uint32_t steps_of(const AttendArgs &a, const SeqInfo &s, uint32_t tile) {
     const uint32_t r0 = tile * kTileRows, r1 = min(r0 + kTileRows, rows_of(a, s));
-    return max((span_of(a, s, r0, r1).nb + 1) / 2, 1u);
+    return max(steps_between(a, position_of(a, s, r0), position_of(a, s, r1 - 1)).n, 1u);
 }
 
 __device__ __forceinline__ TileList tiles_in(const AttendArgs &a, const SeqInfo &s) {
@@ -744,10 +885,9 @@ __device__ __forceinline__ TileList tiles_in(const AttendArgs &a, const SeqInfo 
     const int32_t x = max(first + (int32_t)token_of(a, kTileRows - 1), 0);
     const int32_t y = max(first + (int32_t)token_of(a, l.tiles * kTileRows - 1), 0);
     l.pair = (uint32_t)(x + y + 1) / 64 + 2;
-    if (a.window) {  // a tile's blocks: the sinks', and those from its first row's window to its last row
+    if (a.window) {  // a tile's steps: the sinks', and those from its first row's window to its last row
         const uint32_t tokens = token_of(a, kTileRows + a.group - 2) + 1;
-        const uint32_t blocks = ((uint32_t)a.sinks + kKvBlock - 1) / kKvBlock + ((uint32_t)a.window + tokens) / kKvBlock + 2;
-        l.pair = min(l.pair, 2 * ((blocks + 1) / 2));
+        l.pair = min(l.pair, 2 * (((uint32_t)a.sinks + kStep - 1) / kStep + ((uint32_t)a.window + tokens) / kStep + 2));
     }
     l.middle = l.tiles % 2 ? steps_of(a, s, l.tiles / 2) : 0;
     l.head = l.tiles / 2 * l.pair + l.middle;
@@ -780,64 +920,118 @@ struct RowShare {
     }
 };
 
+// The end of a phase: what was put into the LDS is there, loads from memory go on.
+__device__ __forceinline__ void phase_end() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // Steps [u0, u1) of one tile of one head.
+//
+// Two groups of four wavefronts, one of each on every SIMD, half a step apart: while one group's matrix instructions run (the
+// output of the step before, the scores of this one), the other works out its weights on the vector unit.  A phase ends at
+// a barrier.  With phases counted from 0, the first group's matrix phase of step u0 + t is phase 2 t, its vector phase
+// 2 t + 1; the second group's are one later.  Step t's keys are read in phases 2 t and 2 t + 1, its values in 2 t + 2 and
+// 2 t + 3, both from one of two buffers.  Both groups store their parts of keys t + 1 and values t in matrix phase t (phases
+// 2 t and 2 t + 1): after the last read of what lay there (keys t - 1 and values t - 2: phase 2 t - 1) and before phase 2 t + 2
+// reads them.  Storing, and asking for the next, is a matter of the matrix phase because there the other units are idle.
 template <int KIND, int D>
 __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t seq, const SeqInfo &s, uint32_t head, uint32_t tile,
                                                   uint32_t u0, uint32_t u1, bool whole, float *slot, uint8_t *lds) {
     const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
     const uint32_t t0 = tile * kTileRows, t1 = min(t0 + kTileRows, rows_of(a, s));
-    const Span span = span_of(a, s, t0, t1);
+    const Steps steps = steps_between(a, position_of(a, s, t0), position_of(a, s, t1 - 1));
     const uint32_t r0 = t0 + wave * 32, r1 = min(r0 + 32, t1);
     const bool any = r0 < r1;
-    const Span own = any ? span_of(a, s, r0, r1) : span;
     const Queries<D> q = load_queries<D>(a, s, head, r0 + col, t1);
-    const int32_t pos = s.len - s.n + (int32_t)token_of(a, r0 + col);
+    const int32_t pos = position_of(a, s, r0 + col);
+    // the wavefront's rows stand at p_lo .. p_hi
+    const int32_t p_lo = position_of(a, s, any ? r0 : t0), p_hi = any ? position_of(a, s, r1 - 1) : -1;
     Running<D> run;
     run.clear();
 
-    const uint32_t last = min(u1, (span.nb + 1) / 2);
-    const auto place = [&](uint32_t i, bool &gone) -> const uint8_t * {
-        const uint32_t blk = span.block(min(i, span.nb - 1));
-        const uint32_t page = uniform(page_of(a.batch, a.cache, seq, blk));
-        gone = page == kNoPage;
-        return block_at<KIND, D>(a.cache, gone ? 0 : page, head, blk);
-    };
+    const uint32_t last = min(u1, steps.n);
+    const bool second = wave >= kRowWaves / 2;
     Stage<KIND, D> stage;
-    bool gone[2] = {false, false}, lost = false;
-    if (u0 < last) {
-        const uint8_t *b0 = place(2 * u0, gone[0]), *b1 = place(2 * u0 + 1, gone[1]);
-        stage.fetch(b0, b1);
-    }
-    const auto held = [&](int32_t kb, bool g) { return g ? 0u : bits(0, s.len - kb); };
-    __syncthreads();  // (the LDS is free of the piece before)
-    for (uint32_t st = u0; st < last; ++st) {
-        uint8_t *buf = lds + (st & 1) * (256 * D);
-        const bool g0 = gone[0], g1 = gone[1] || 2 * st + 1 >= span.nb;
-        const int32_t kb0 = (int32_t)(span.block(2 * st) * kKvBlock);
-        const int32_t kb1 = (int32_t)(span.block(min(2 * st + 1, span.nb - 1)) * kKvBlock);
-        stage.store(buf, held(kb0, g0), held(kb1, g1));
-        lost = lost || g0 || gone[1];
-        __syncthreads();
-        if (st + 1 < last) {
-            const uint8_t *b0 = place(2 * st + 2, gone[0]), *b1 = place(2 * st + 3, gone[1]);
-            stage.fetch(b0, b1);
-        }
-        // a wavefront none of whose rows sees a key of either block has nothing to do in this step
-        const int32_t lo = a.window ? own.p_lo - a.window + 1 : 0;
-        const auto seen = [&](int32_t kb) { return kb <= own.p_hi && (kb + 31 >= lo || kb < a.sinks); };
-        if (!any || !((seen(kb0) && !g0) || (seen(kb1) && !g1))) continue;
-        const bool edge = g0 || g1 || !all_visible(a, own, kb0) || !all_visible(a, own, kb1);
+    PageRun table(a.batch, seq);
+    bool lost = false;  // whether a block was on no page of the cache (page 0 then stands for it, and the rows are done again)
+    const uint32_t last_block = s.len > 0 ? (uint32_t)(s.len - 1) / kKvBlock : 0;
+    const auto buffer = [&](uint32_t st) { return lds + (st & 1) * (256 * D); };
+    const auto first_block = [&](uint32_t st) { return (uint32_t)steps.first_key(min(st, last - 1)) / kKvBlock; };
+    const auto at_block = [&](uint32_t blk) {
+        const uint32_t x = table.page_of(a.cache, blk);
+        lost = lost || x == kNoPage;
+        return block_at<KIND, D>(a.cache, x == kNoPage ? 0 : x, head, blk);
+    };
+    Blocks kp{}, vp{};
+    const auto ask = [&](uint32_t st) {  // keys of step st (the last one's again behind it), values of the step asked for before
+        vp = kp;
+        const uint32_t blk = first_block(st);
+        kp.b0 = at_block(blk);
+        kp.b1 = at_block(min(blk + 1, last_block));  // (none behind the sequence's end)
+        stage.fetch(kp, vp);
+    };
+    // what is staged: keys of step ks, values of the step before
+    const auto put = [&](uint32_t ks) { stage.store(buffer(ks), buffer(ks - 1)); };
+    const auto clear = [&](uint32_t ks) {
+        const int32_t kb = (int32_t)(first_block(ks - 1) * kKvBlock);
+        if (kb + (int32_t)kStep > s.len) stage.clear(bits(0, s.len - kb), bits(0, s.len - kb - 32));
+    };
+    const auto hold = [&](uint32_t st) { table.hold(a.batch, a.cache, first_block(st)); };
+    // steps [clean0, clean1) need no mask for the wavefront's rows
+    const uint32_t clean0 = a.window ? steps.s1 + (p_hi - a.window < 0 ? 0u : max((uint32_t)(p_hi - a.window) / kStep + 1, steps.w0) - steps.w0) : 0;
+    const uint32_t clean1 = p_lo + 1 < (int32_t)kStep ? 0 : steps.s1 + max((uint32_t)(p_lo + 1) / kStep, steps.w0) - steps.w0;
 
-        const u32x4 *kv = reinterpret_cast<const u32x4 *>(buf);
-        constexpr int kBlk = 8 * D;  // 16-byte pieces of a block: keys, then values
-        f32x16_p acc0 = splat16(0.0f), acc1 = acc0;
+    constexpr int kBlk = 8 * D;  // 16-byte pieces of a block: keys, then values
+    f32x16_p acc0, acc1;
+    u32x4 p[4];
+    const auto output = [&](uint32_t st) {
+        const u32x4 *kv = reinterpret_cast<const u32x4 *>(buffer(st)) + 4 * D + lane;
+#pragma unroll
+        for (int s2 = 0; s2 < 4; ++s2)
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+                run.o[db] = mfma(kv[(s2 / 2) * kBlk + ((s2 % 2) * (D / 32) + db) * 64], p[s2], run.o[db]);
+    };
+    const auto scores = [&](uint32_t st) {
+        const u32x4 *kv = reinterpret_cast<const u32x4 *>(buffer(st)) + lane;
+        acc0 = acc1 = splat16(0.0f);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-            acc0 = mfma(kv[k * 64 + lane], q.f[k], acc0);
-            acc1 = mfma(kv[kBlk + k * 64 + lane], q.f[k], acc1);
+            acc0 = mfma(kv[k * 64], q.f[k], acc0);
+            acc1 = mfma(kv[kBlk + k * 64], q.f[k], acc1);
         }
-        if (edge) {
-            const uint32_t s0 = g0 ? 0u : seen_keys(a, pos, pos, kb0) >> (4 * h), s1 = g1 ? 0u : seen_keys(a, pos, pos, kb1) >> (4 * h);
+    };
+    __syncthreads();  // (the LDS is free of the piece before)
+    if (u0 < last) {
+        hold(u0);
+        kp.b0 = at_block(first_block(u0));  // (the first step's values go with its keys, unread)
+        kp.b1 = kp.b0;
+        ask(u0);
+        stage.convert();
+        put(u0);
+        hold(u0 + 1);
+        ask(u0 + 1);
+        hold(u0 + 2);
+        clear(u0 + 1);
+        stage.convert();
+        __syncthreads();
+        if (second) phase_end();
+        put(u0 + 1);
+        ask(u0 + 2);
+        scores(u0);
+        phase_end();
+    }
+    for (uint32_t st = u0; st < last; ++st) {
+        // ---- vector phase
+        hold(st + 3);
+        clear(st + 2);
+        stage.convert();
+        if (st < clean0 || st >= clean1) {
+            const int32_t kb = steps.first_key(st);
+            const uint32_t s0 = seen_keys(a, pos, pos, kb) >> (4 * h), s1 = seen_keys(a, pos, pos, kb + 32) >> (4 * h);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 acc0[e] = s0 >> ((e & 3) + 8 * (e >> 2)) & 1 ? acc0[e] : kNone;
@@ -849,7 +1043,6 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         for (int e = 0; e < 16; ++e) best = most(best, most(acc0[e], acc1[e]));
         run.raise(max_halves(best) * a.scale_log2);
         const float base = run.base();
-        u32x4 p[4];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
             const float x0 = exp2_fast(acc0[e] * a.scale_log2 - base), x1 = exp2_fast(acc0[e + 1] * a.scale_log2 - base);
@@ -858,16 +1051,25 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
             p[e / 8][e / 2 % 4] = bf16_pair(x0, x1);
             p[2 + e / 8][e / 2 % 4] = bf16_pair(y0, y1);
         }
-#pragma unroll
-        for (int s2 = 0; s2 < 4; ++s2)
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db)
-                run.o[db] = mfma(kv[(s2 / 2) * kBlk + 4 * D + ((s2 % 2) * (D / 32) + db) * 64 + lane], p[s2], run.o[db]);
+        phase_end();
+        // ---- matrix phase (behind the last step: the scores of what lies there, for nothing)
+        __builtin_amdgcn_s_setprio(1);
+        put(st + 2);
+        ask(st + 3);
+        output(st);
+        scores(st + 1);
+        __builtin_amdgcn_s_setprio(0);
+        phase_end();
     }
-    if (lost && threadIdx.x == 0) report_bad_index(a.batch);
+    if (u0 < last && !second) phase_end();  // (the second group's last phase)
+    if (lost) {
+        if (threadIdx.x == 0) report_bad_index(a.batch);
+        run.l = __builtin_nanf("");  // (the rows will be found to be no numbers, and done again)
+    }
     const float l = run.l + other_half(run.l);
-    if (r0 + col >= t1) return;
+    const bool mine = r0 + col < t1;
     if (!whole) {
+        if (!mine) return;
         float *o = slot + (r0 - t0 + col) * D;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
@@ -883,22 +1085,33 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         return;
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const uint32_t tok = token_of(a, r0 + col), gh = head * a.group + r0 + col - tok * a.group;
-    uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
+    float check = 0.0f;
+    if (mine) {
+        const uint32_t tok = token_of(a, r0 + col), gh = head * a.group + r0 + col - tok * a.group;
+        uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+        for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            u32x2 w = {bf16_pair(run.o[db][4 * k] * inv, run.o[db][4 * k + 1] * inv),
-                       bf16_pair(run.o[db][4 * k + 2] * inv, run.o[db][4 * k + 3] * inv)};
-            *reinterpret_cast<u32x2 *>(dst + 32 * db + 8 * k + 4 * h) = w;
-        }
-    if (a.lse && h == 0)
-        a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = run.m == kNone ? kNone : (run.m + log2f(l)) * 0.6931471805599453f;
+            for (int k = 0; k < 4; ++k) {
+                float y[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    y[c] = run.o[db][4 * k + c] * inv;
+                    check = fmaf(y[c], 0.0f, check);  // (a NaN once one of them is no number)
+                }
+                u32x2 w = {bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3])};
+                *reinterpret_cast<u32x2 *>(dst + 32 * db + 8 * k + 4 * h) = w;
+            }
+        if (a.lse && h == 0)
+            a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = run.m == kNone ? kNone : (run.m + log2f(l)) * 0.6931471805599453f;
+    }
+    const uint64_t again = __builtin_amdgcn_ballot_w64(check != check);
+    for (uint32_t rows = (uint32_t)again | (uint32_t)(again >> 32); rows; rows &= rows - 1)
+        attend_one_row<KIND, D>(a, seq, s, head, r0 + (uint32_t)__builtin_ctz(rows));
 }
 
 template <int KIND, int D>
-__global__ __launch_bounds__(kRowThreads, D == 128 ? 2 : 4) void attend_rows_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kRowThreads, 2 * row_groups(KIND, D)) void attend_rows_kernel(AttendArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     uint32_t *word = reinterpret_cast<uint32_t *>(lds);
     // Workgroups go to the eight XCDs in turn, and each has an L2 of its own: an XCD takes a contiguous run of the list, so
@@ -945,7 +1158,7 @@ __global__ __launch_bounds__(kRowThreads, D == 128 ? 2 : 4) void attend_rows_ker
 }
 
 // 32 rows of the tile that the cut before workgroup blockIdx.x + 1 goes through: the sum of its parts.
-template <int D>
+template <int KIND, int D>
 __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uint32_t workers) {
     __shared__ uint32_t word[10];
     const uint32_t k = blockIdx.x + 1;
@@ -970,6 +1183,8 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
     uint32_t w1 = (at + t.places - 1) / cuts.share;
     if (w1 > k && cuts.cut(w1 * cuts.share - at, t.places) == t.places) --w1;
     constexpr uint32_t kLanes = D / 4;
+    if (threadIdx.x == 0) word[0] = 0;  // rows that are no numbers, a bit each
+    __syncthreads();
     const uint32_t d = threadIdx.x % kLanes * 4;
     for (uint32_t r = r0 + threadIdx.x / kLanes; r < r1; r += 256 / kLanes) {
         float m = kNone, l = 0.0f;
@@ -990,7 +1205,12 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
         *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
         if (a.lse && d == 0)
             a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
+        if (no_number(acc[0] * inv + acc[1] * inv + (acc[2] * inv + acc[3] * inv))) atomicOr(word, 1u << (r - r0));
     }
+    __syncthreads();
+    const uint32_t again = uniform(word[0]);
+    for (uint32_t r = r0 + uniform(threadIdx.x >> 6); r < r1; r += 4)
+        if (again >> (r - r0) & 1) attend_one_row<KIND, D>(a, f.seq, s, head, r);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -1002,7 +1222,7 @@ struct AttendPlan {
 };
 
 // `longest`, `new_longest`: the caller's bounds on the lengths.  They choose kernels; the results do not rest on them.
-static int plan_attend(const KvView &v, const KvBatch &b, uint32_t head_dim, uint32_t group, int32_t window, int32_t sinks,
+static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_t head_dim, uint32_t group, int32_t window, int32_t sinks,
                        uint32_t new_longest, uint32_t longest, AttendPlan *p) {
     uint32_t cus = 1;
     if (int rc = cu_count(&cus)) return rc;
@@ -1017,8 +1237,7 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t head_dim, uin
     if (items > 0x7FFFFF00ull) return fail(CI_ERR_ARG, "ci_paged_attention: too many rows for one call");
     p->items = (uint32_t)items;
     if (p->many) {
-        // as many as are resident: two wavefronts per SIMD for heads of 128, four for heads of 64
-        p->workers = p->grid = ((head_dim == 128 ? 512 : 1024) * cus / kRowThreads + 7) / 8 * 8;
+        p->workers = p->grid = (cus * row_groups(kind, head_dim) + 7) / 8 * 8;
         p->work_bytes = (size_t)p->workers * 2 * kTileRows * (head_dim + 2) * sizeof(float);
         return CI_OK;
     }
@@ -1037,7 +1256,7 @@ static int launch_split(const AttendArgs &a, const AttendPlan &p, hipStream_t s)
     CI_KV_LAUNCH((attend_split_kernel<KIND, D, RP>), dim3(p.grid), dim3(256), split_lds(D), s, a);
     CI_LAUNCH_CHECK("attend_split_kernel");
     if (!p.whole) {
-        CI_KV_LAUNCH((attend_join_kernel<D, RP>), dim3(p.items, RP), dim3(256), 0, s, a, p.workers);
+        CI_KV_LAUNCH((attend_join_kernel<KIND, D, RP>), dim3(p.items, RP), dim3(256), 0, s, a, p.workers);
         CI_LAUNCH_CHECK("attend_join_kernel");
     }
     return CI_OK;
@@ -1050,7 +1269,7 @@ static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s
         CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(kRowThreads), rows_lds(D), s, a);
         CI_LAUNCH_CHECK("attend_rows_kernel");
         if (p.workers > 1) {
-            CI_KV_LAUNCH((attend_rows_join_kernel<D>), dim3(p.workers - 1, kTileRows / 32), dim3(256), 0, s, a, p.workers);
+            CI_KV_LAUNCH((attend_rows_join_kernel<KIND, D>), dim3(p.workers - 1, kTileRows / 32), dim3(256), 0, s, a, p.workers);
             CI_LAUNCH_CHECK("attend_rows_join_kernel");
         }
         return CI_OK;
@@ -1087,7 +1306,7 @@ extern "C" size_t ci_paged_attention_workspace_bytes(const ci_kv_cache *cache, c
     AttendPlan p;
     if (check_attend("ci_paged_attention_workspace_bytes", cache, batch, q_heads, window, sinks, &v, &b)) return 0;
     if (b.seqs == 0 || b.tokens == 0) return 0;
-    if (plan_attend(v, b, cache->head_dim, q_heads / v.kv_heads, window, sinks, max_query_len ? max_query_len : b.tokens,
+    if (plan_attend(v, b, cache->kind, cache->head_dim, q_heads / v.kv_heads, window, sinks, max_query_len ? max_query_len : b.tokens,
                     max_seq_len ? max_seq_len : b.table_width << (v.page_shift + 5), &p))
         return 0;
     return p.work_bytes;
@@ -1119,7 +1338,7 @@ extern "C" int ci_paged_attention(const ci_kv_cache *cache, const ci_kv_batch *b
     a.window = window < (1 << 30) ? window : 1 << 30;  // (no sequence is longer: sums of positions stay in 32 bits)
     a.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
     AttendPlan p;
-    if (int rc = plan_attend(a.cache, a.batch, cache->head_dim, a.group, window, sinks, max_query_len ? max_query_len : a.batch.tokens,
+    if (int rc = plan_attend(a.cache, a.batch, cache->kind, cache->head_dim, a.group, window, sinks, max_query_len ? max_query_len : a.batch.tokens,
                              max_seq_len ? max_seq_len : a.batch.table_width << (a.cache.page_shift + 5), &p))
         return rc;
     if (p.work_bytes && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < p.work_bytes))

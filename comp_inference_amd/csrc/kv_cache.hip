@@ -377,7 +377,8 @@ int check_kv_cache(const char *who, const ci_kv_cache *c, KvView *v) {
                     (unsigned long long)need);
     uint32_t shift = 0;
     while ((kKvBlock << shift) < c->page_size) ++shift;
-    *v = KvView{static_cast<uint8_t *>(c->d_data), c->num_pages, shift, c->kv_heads};
+    *v = KvView{static_cast<uint8_t *>(c->d_data), c->num_pages, shift, c->kv_heads,
+                c->page_size / kKvBlock * block_bytes(c->kind, c->head_dim)};
     return CI_OK;
 }
 

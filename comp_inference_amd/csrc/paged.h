@@ -64,6 +64,7 @@ __device__ __forceinline__ uint32_t nibble_shift(uint32_t e) { return 4 * (e >> 
 struct KvView {
     uint8_t *data;
     uint32_t num_pages, page_shift, kv_heads;  // page_shift: log2 of the blocks of a page
+    uint32_t head_bytes;                       // bytes of a page that belong to one head
 };
 
 struct KvBatch {
@@ -111,10 +112,32 @@ __device__ __forceinline__ uint32_t page_of(const KvBatch &b, const KvView &v, u
     return page < v.num_pages ? page : kNoPage;
 }
 
+// The same for a wavefront that walks through a sequence: 64 entries of the table at a time, one in each lane, so that a
+// step finds its page without waiting for memory.
+struct PageRun {
+    const int32_t *row;
+    uint32_t held, pages;  // which 64 entries; this lane's
+    __device__ __forceinline__ PageRun(const KvBatch &b, uint32_t seq) : row(b.table + (uint64_t)seq * b.table_stride), held(kNoPage), pages(0) {}
+    // makes sure that the entry of block `blk` is among those held
+    __device__ __forceinline__ void hold(const KvBatch &b, const KvView &v, uint32_t blk) {
+        const uint32_t which = blk >> v.page_shift >> 6;
+        if (which != held) {
+            held = which;
+            const uint32_t at = held * 64 + (threadIdx.x & 63);
+            pages = at < b.table_width ? (uint32_t)row[at] : kNoPage;
+        }
+    }
+    // the page of a block whose entry is held
+    __device__ __forceinline__ uint32_t page_of(const KvView &v, uint32_t blk) const {
+        const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)pages, (int)((blk >> v.page_shift) & 63));
+        return page < v.num_pages ? page : kNoPage;
+    }
+};
+
 template <int KIND, int D>
 __device__ __forceinline__ uint8_t *block_at(const KvView &v, uint32_t page, uint32_t head, uint32_t blk) {
-    const uint64_t index = (((uint64_t)page * v.kv_heads + head) << v.page_shift) + (blk & ((1u << v.page_shift) - 1));
-    return v.data + index * KvBlock<KIND, D>::kBytes;
+    return v.data + (uint64_t)page * (v.head_bytes * v.kv_heads) + (uint64_t)(head * v.head_bytes) +
+           (blk & ((1u << v.page_shift) - 1)) * KvBlock<KIND, D>::kBytes;  // (a page is below 4 GiB)
 }
 
 // Exclusive prefix sum over the threads of a workgroup (up to eight wavefronts); `total` gets the sum.  `part` holds eight

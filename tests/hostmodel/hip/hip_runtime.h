@@ -75,6 +75,10 @@ CI_SIM_MINMAX(double)
 #define __builtin_amdgcn_s_sleep(n) sim::yield()
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, x, y, z) sim::mfma_32x32x16_bf16((a), (b), (c))
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __builtin_amdgcn_s_barrier() sim::syncthreads()
+#define __builtin_amdgcn_sched_barrier(mask) ((void)0)
+#define __builtin_amdgcn_s_setprio(n) ((void)0)
+
 #define __shfl(v, src, width) sim::shfl((int)(v), (int)(src), (int)(width))
 #define __shfl_up(v, d, width) sim::shfl_up((int)(v), (unsigned)(d), (int)(width))
 
