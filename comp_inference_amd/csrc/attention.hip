@@ -728,6 +728,7 @@ constexpr uint32_t kRowWaves = 8, kRowThreads = 64 * kRowWaves, kTileRows = 32 *
 constexpr uint32_t rows_lds(int D) { return 2 * 2 * 128 * D; }  // two buffers of two blocks, keys and values in bf16
 // Workgroups resident on a CU: registers allow two wavefronts per SIMD, four for heads of 64 in bf16.
 constexpr uint32_t row_groups(uint32_t kind, uint32_t dim) { return kind == CI_KV_BF16 && dim == 64 ? 2 : 1; }
+constexpr uint32_t kWholeSteps = 32;                             // a tile of up to so many steps is never cut
 constexpr uint32_t kLeastShare = 16;                             // steps (of 64 keys) worth a workgroup
 
 struct Blocks {  // the two blocks of a step
@@ -762,7 +763,6 @@ struct Stage<CI_KV_BF16, D> {
         for (int i = 0; i < N; ++i)
             if (is_value(i)) x[i] = keep_seen(x[i], (i < N / 2 ? held0 : held1) >> (16 * ((piece(i) - 4 * D) / (2 * D)) + 4 * h), 0);
     }
-    __device__ __forceinline__ void convert() {}
     // keys to buffer `kb`, values to buffer `vb`
     __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb) const {
 #pragma unroll
@@ -777,9 +777,8 @@ struct Stage<CI_KV_BF16, D> {
 template <int D>
 struct Stage<CI_KV_INT4, D> {
     static constexpr int N = D / 64;  // pieces of the keys of a block
-    u32x4 x, y[4];
+    u32x4 x;
     uint32_t own, pair[16 / N];  // (step, low): of the lane's key; of its tokens in the values (16 for heads of 64, 8 for 128)
-    uint32_t held = 0xFFFFFFFFu;  // tokens of the piece's block that are there
     static __device__ __forceinline__ uint32_t unit() { return uniform(threadIdx.x >> 6); }
     static __device__ __forceinline__ bool idle() { return unit() >= 4 * N; }
     static __device__ __forceinline__ uint32_t block() { return unit() / (2 * N) & 1; }
@@ -802,26 +801,12 @@ struct Stage<CI_KV_INT4, D> {
             for (int e = 0; e < 4; ++e) pair[c + e] = w[e];
         }
     }
-    __device__ __forceinline__ void clear(uint32_t held0, uint32_t held1) { held = block() ? held1 : held0; }
-    __device__ __forceinline__ void convert() {
-        if (idle()) return;
-        const uint32_t lane = threadIdx.x & 63;
-        if (values()) {
+    // (a value of a token that is not there: step 0, low 0)
+    __device__ __forceinline__ void clear(uint32_t held0, uint32_t held1) {
+        const uint32_t here = (block() ? held1 : held0) >> (4 * ((threadIdx.x >> 5) & 1) + (N == 2 ? 16 * index() : 0));
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float step[8], low[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) step[e] = bf16_lo(pair[(N == 2 ? 0 : c / 2 * 8) + e]), low[e] = bf16_hi(pair[(N == 2 ? 0 : c / 2 * 8) + e]);
-                y[c] = eight(x[c], step, low);
-                if (held != 0xFFFFFFFFu) y[c] = keep_seen(y[c], held >> (4 * (lane >> 5) + 16 * (N == 2 ? index() : c / 2)), 0);
-            }
-        } else {
-            float step[8], low[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) step[e] = bf16_lo(own), low[e] = bf16_hi(own);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) y[c] = eight(x[c], step, low);
-        }
+        for (uint32_t c = 0; c < 16 / N; ++c)
+            if (!(here >> (16 * (c / 8) + value_token(0, 0, c % 8)) & 1)) pair[c] = 0;
     }
     static __device__ __forceinline__ u32x4 eight(uint32_t word, const float (&step)[8], const float (&low)[8]) {
         const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;  // codes 0, 4, 1, 5 and 2, 6, 3, 7, a byte each
@@ -835,10 +820,19 @@ struct Stage<CI_KV_INT4, D> {
         return r;
     }
     __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb) const {
-        if (idle()) return;
+        if (N == 1 && idle()) return;
         u32x4 *dst = reinterpret_cast<u32x4 *>((values() ? vb : kb) + block() * 128 * D + values() * 64 * D) + index() * 256 + (threadIdx.x & 63);
+        const uint32_t mask = 0u - values();  // (keys and values by the same instructions: a branch would stop the matrix unit)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) dst[c * 64] = y[c];
+        for (int c = 0; c < 4; ++c) {
+            float step[8], low[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t w = (pair[(N == 2 ? 0 : c / 2 * 8) + e] & mask) | (own & ~mask);
+                step[e] = bf16_lo(w), low[e] = bf16_hi(w);
+            }
+            dst[c * 64] = eight(x[c], step, low);
+        }
     }
 };
 
@@ -914,8 +908,9 @@ struct RowShare {
         share = max((total + workers - 1) / workers, kLeastShare);
         slack = max(share / 16, 7u);
     }
-    // where a cut `off` places behind a tile's begin (0 < off < places, or 0) goes
+    // where a cut `off` places behind a tile's begin (0 < off < places, or 0) goes; a tile of few steps is never cut
     __device__ __forceinline__ uint32_t cut(uint32_t off, uint32_t places) const {
+        if (places <= kWholeSteps) return 2 * off < places ? 0 : places;
         return off <= slack ? 0 : places - off <= slack ? places : off;
     }
 };
@@ -1010,13 +1005,11 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         kp.b0 = at_block(first_block(u0));  // (the first step's values go with its keys, unread)
         kp.b1 = kp.b0;
         ask(u0);
-        stage.convert();
         put(u0);
         hold(u0 + 1);
         ask(u0 + 1);
         hold(u0 + 2);
         clear(u0 + 1);
-        stage.convert();
         __syncthreads();
         if (second) phase_end();
         put(u0 + 1);
@@ -1028,7 +1021,6 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         // ---- vector phase
         hold(st + 3);
         clear(st + 2);
-        stage.convert();
         if (st < clean0 || st >= clean1) {
             const int32_t kb = steps.first_key(st);
             const uint32_t s0 = seen_keys(a, pos, pos, kb) >> (4 * h), s1 = seen_keys(a, pos, pos, kb + 32) >> (4 * h);
@@ -1054,9 +1046,13 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         phase_end();
         // ---- matrix phase (behind the last step: the scores of what lies there, for nothing)
         __builtin_amdgcn_s_setprio(1);
+        // (in the order that keeps the matrix unit fed: turning codes into values takes the vector unit a while, and runs
+        // beside the first half's matrix instructions; copies are best out of the way first.  The other way round: a 4-bit
+        // prompt part 892 instead of 816 us, a bf16 prompt 658 instead of 552)
+        if (KIND != CI_KV_BF16) output(st);
         put(st + 2);
         ask(st + 3);
-        output(st);
+        if (KIND == CI_KV_BF16) output(st);
         scores(st + 1);
         __builtin_amdgcn_s_setprio(0);
         phase_end();
@@ -1116,8 +1112,25 @@ __global__ __launch_bounds__(kRowThreads, 2 * row_groups(KIND, D)) void attend_r
     uint32_t *word = reinterpret_cast<uint32_t *>(lds);
     // Workgroups go to the eight XCDs in turn, and each has an L2 of its own: an XCD takes a contiguous run of the list, so
     // that the tiles of a head read its keys and values through one L2.
-    const uint32_t worker = (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
     Found f;
+    bool bad;
+    if (a.whole) {  // one tile each, those with the most keys of a head first
+        const auto items = [&](uint32_t i) {
+            bool x;
+            return tiles_in(a, load_seq(a.batch, a.cache, i, x)).tiles * a.cache.kv_heads;
+        };
+        const auto mine = [&](uint32_t total) {
+            const uint32_t run = (total + 7) / 8, k = blockIdx.x >> 3;
+            return k < run ? (blockIdx.x & 7) * run + k : 0xFFFFFFFFu;
+        };
+        if (!locate(a.batch.seqs, items, mine, word, f)) return;
+        const SeqInfo s = load_seq(a.batch, a.cache, f.seq, bad);
+        if (bad && threadIdx.x == 0) report_bad_index(a.batch);
+        const uint32_t tiles = tiles_in(a, s).tiles, head = (f.target - f.begin) / tiles;
+        attend_rows_piece<KIND, D>(a, f.seq, s, head, tiles - 1 - (f.target - f.begin) % tiles, 0, 0xFFFFFFFFu, true, nullptr, lds);
+        return;
+    }
+    const uint32_t worker = (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
     const auto weight = [&](uint32_t i) {
         bool x;
         return tiles_in(a, load_seq(a.batch, a.cache, i, x)).head * a.cache.kv_heads;
@@ -1126,7 +1139,6 @@ __global__ __launch_bounds__(kRowThreads, 2 * row_groups(KIND, D)) void attend_r
     const RowShare cuts(f.total, gridDim.x);
     uint32_t seq = f.seq, base = f.begin;  // of the list, where the sequence begins
     const uint32_t end = min(f.target + cuts.share, f.total);
-    bool bad;
     SeqInfo s = load_seq(a.batch, a.cache, seq, bad);
     TileList list = tiles_in(a, s);
     uint32_t place = f.target - base;
@@ -1179,6 +1191,7 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
     if (moved == 0 || moved == t.places) return;                                      // not cut here
     if (off > cuts.share && cuts.cut(off - cuts.share, t.places) != 0) return;  // cut before: joined there
     const uint32_t t0 = t.tile * kTileRows, r0 = t0 + blockIdx.y * 32, r1 = min(r0 + 32, rows_of(a, s));
+    if (r0 >= r1) return;
     const uint32_t w0 = k - 1;
     uint32_t w1 = (at + t.places - 1) / cuts.share;
     if (w1 > k && cuts.cut(w1 * cuts.share - at, t.places) == t.places) --w1;
@@ -1238,7 +1251,14 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     p->items = (uint32_t)items;
     if (p->many) {
         p->workers = p->grid = (cus * row_groups(kind, head_dim) + 7) / 8 * 8;
-        p->work_bytes = (size_t)p->workers * 2 * kTileRows * (head_dim + 2) * sizeof(float);
+        // tiles of few steps: one workgroup each, handed out by the hardware, and nothing to join (ragged prompts of up to 6001
+        // tokens under a window of 1000: 153 us in shares, 124 whole)
+        uint64_t keys = longest;
+        const uint64_t reach = (uint64_t)window + sinks + kTileRows / group + 3 * kStep;
+        if (window && reach < keys) keys = reach;
+        p->whole = keys <= kWholeSteps * kStep;
+        if (p->whole) p->grid = (p->items + 7) / 8 * 8;
+        else p->work_bytes = (size_t)p->workers * 2 * kTileRows * (head_dim + 2) * sizeof(float);
         return CI_OK;
     }
     uint64_t keys = longest;
@@ -1268,7 +1288,7 @@ static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s
         CI_ALLOW_FULL_LDS((attend_rows_kernel<KIND, D>));
         CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(kRowThreads), rows_lds(D), s, a);
         CI_LAUNCH_CHECK("attend_rows_kernel");
-        if (p.workers > 1) {
+        if (!p.whole && p.workers > 1) {
             CI_KV_LAUNCH((attend_rows_join_kernel<KIND, D>), dim3(p.workers - 1, kTileRows / 32), dim3(256), 0, s, a, p.workers);
             CI_LAUNCH_CHECK("attend_rows_join_kernel");
         }

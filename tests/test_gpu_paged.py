@@ -476,3 +476,37 @@ def test_results_do_not_hang_on_timing():
     first = ci.paged_attention(f.q.to(DEV), *f.args(rows=False))
     for _ in range(5):
         assert torch.equal(first, ci.paged_attention(f.q.to(DEV), *f.args(rows=False)))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int4"])
+@pytest.mark.parametrize("lens,news,longest", [([90], [90], 0), ([40, 300], [3, 6], 2), ([1500], [1500], 0), ([900], [2], 2)])
+def test_what_a_row_does_not_see_may_be_anything(kind, lens, news, longest):
+    """Keys and values of infinities and NaN at tokens that some rows of a tile see and others do not: those others get what
+    they get without them, and the rows that see a NaN are NaN."""
+    ci = _ci()
+    heads, G, D, window, sinks = 4, 2, 64, 20, 1
+    f = Filled(lens, news, heads, G, D, kind, seed=61)
+    where = [l - n + n // 2 for l, n in zip(lens, news)]  # a token in the middle of the new ones
+    k, v = [x.clone() for x in f.k], [x.clone() for x in f.v]
+    for b, t in enumerate(where):
+        v[b][t] = torch.tensor([math.inf, -math.inf, math.nan, 1.0] * (D // 4), dtype=torch.bfloat16)
+        if b % 2:
+            k[b][t] = math.nan
+    whole = torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32).to(DEV)
+    ci.paged_kv_append(f.cache, torch.cat(k).to(DEV), torch.cat(v).to(DEV), f.table, f.seq, whole)
+    for kw in ({}, dict(window=window, sinks=sinks)):
+        want, _, bound = f.expect(values_rounded=kind == "int4", **kw)
+        plain = f.expect(**kw)
+        got = ci.paged_attention(f.q.to(DEV), *f.args(), max_query_len=longest, **kw).double().cpu()
+        at = 0
+        for l, n, t in zip(lens, news, where):
+            p = torch.arange(l - n, l)
+            sees = (p >= t) & ((p - t < window) | (t < sinks)) if kw else p >= t
+            rows = slice(at, at + n)
+            clean = got[rows][~sees]
+            off = torch.minimum((clean - want[rows][~sees]).abs() - bound[rows][~sees],
+                                (clean - plain[0][rows][~sees]).abs() - plain[2][rows][~sees])
+            assert not len(off) or float(off.max()) <= 0, (kw, float(off.max()))
+            assert not torch.isfinite(got[rows][sees][..., 2::4]).any()  # (the channels whose value is NaN)
+            at += n
+    assert ci.device_status() == 0
