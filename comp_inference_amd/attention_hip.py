@@ -98,42 +98,48 @@ def _elsewhere(name: str, t, cache: PagedKVCache):
     return RuntimeError(f"{name} is on {t.device}, the cache on {cache.data.device}")
 
 
+# These checks run in front of every launch of a token loop: each asks a tensor for its properties once, all conditions in
+# one test, and only a call that is refused finds out which one it was.
+
 def _batch(cache: PagedKVCache, index: int, block_table, seq_lens, query_start, tokens: int):
-    """ci_kv_batch by reference.  (These checks run in front of every launch of a token loop: one query per property.)"""
-    seqs, width = seq_lens.numel(), 0
+    """ci_kv_batch by reference."""
+    seqs, start = seq_lens.numel(), None
+    ok = (block_table.dtype is torch.int32 and seq_lens.dtype is torch.int32 and block_table.dim() == 2
+          and seq_lens.dim() == 1 and block_table.get_device() == index and seq_lens.get_device() == index
+          and seq_lens.is_contiguous())
+    if query_start is not None:
+        ok = (ok and query_start.dtype is torch.int32 and query_start.dim() == 1 and query_start.get_device() == index
+              and query_start.numel() == seqs + 1 and query_start.is_contiguous())
+        start = query_start.data_ptr()
+    if ok:
+        (rows, width), (step, inner) = block_table.shape, block_table.stride()
+        if rows == seqs and (start is not None or tokens == seqs) and (inner == 1 or width <= 1) and step >= 0:
+            return C.byref(_Batch(block_table.data_ptr(), step if seqs > 1 else width, width, seq_lens.data_ptr(), start,
+                                  seqs, tokens))
     for name, t, dim in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1), ("query_start", query_start, 1)):
-        if t is None:
-            continue
-        if t.dtype is not torch.int32 or t.dim() != dim:
+        if t is not None and (t.dtype is not torch.int32 or t.dim() != dim):
             raise RuntimeError(f"{name} must be a {dim}-D int32 tensor")
-        if t.get_device() != index:
+        if t is not None and t.get_device() != index:
             raise _elsewhere(name, t, cache)
-    rows, width = block_table.shape
-    if rows != seqs or (query_start is not None and query_start.numel() != seqs + 1):
+    if block_table.shape[0] != seqs or (query_start is not None and query_start.numel() != seqs + 1):
         raise ValueError(f"block_table must have {seqs} rows and query_start {seqs + 1} entries for {seqs} sequences")
     if query_start is None and tokens != seqs:
         raise ValueError(f"without query_start there is one new token per sequence: {tokens} rows, {seqs} sequences")
-    step, inner = block_table.stride()
-    if seqs and (not seq_lens.is_contiguous() or (query_start is not None and not query_start.is_contiguous())
-                 or (width > 1 and inner != 1) or step < 0):
-        raise RuntimeError("seq_lens and query_start must be contiguous, and the rows of block_table")
-    return C.byref(_Batch(block_table.data_ptr(), step if seqs > 1 else width, width, seq_lens.data_ptr(),
-                          None if query_start is None else query_start.data_ptr(), seqs, tokens))
+    raise RuntimeError("seq_lens and query_start must be contiguous, and the rows of block_table")
 
 
 def _rows(name: str, t: torch.Tensor, cache: PagedKVCache, index: int, heads: int | None, tokens: int | None):
     """ci_rows by reference of [tokens, heads, head_dim] in bf16 with unit stride inside a head."""
+    if t.dtype is torch.bfloat16 and t.dim() == 3 and t.get_device() == index:
+        (n, h, d), (row, head, inner), at = t.shape, t.stride(), t.data_ptr()
+        if d == cache.head_dim and (heads is None or h == heads) and (tokens is None or n == tokens):
+            if (inner == 1 and not (at & 15 or (row | head) & 7)) or n == 0 or h == 0:
+                return C.byref(_Rows(at, row, head))
+            raise RuntimeError(f"{name} must have unit stride inside a head, 16-byte aligned rows and strides that are multiples of 8")
+        raise ValueError(f"{name} has shape {(n, h, d)}; the other operands ask for ({tokens}, {heads}, {cache.head_dim})")
     if t.dtype is not torch.bfloat16 or t.dim() != 3:
         raise RuntimeError(f"{name} must be a 3-D bfloat16 tensor [tokens, heads, head_dim]")
-    if t.get_device() != index:
-        raise _elsewhere(name, t, cache)
-    n, h, d = t.shape
-    if d != cache.head_dim or (heads is not None and h != heads) or (tokens is not None and n != tokens):
-        raise ValueError(f"{name} has shape {(n, h, d)}; the other operands ask for ({tokens}, {heads}, {cache.head_dim})")
-    at, (row, head, inner) = t.data_ptr(), t.stride()
-    if (inner != 1 or at % 16 or row % 8 or head % 8) and t.numel():
-        raise RuntimeError(f"{name} must have unit stride inside a head, 16-byte aligned rows and strides that are multiples of 8")
-    return C.byref(_Rows(at, row, head))
+    raise _elsewhere(name, t, cache)
 
 
 def _output(name: str, given, tokens: int, heads: int, cache: PagedKVCache) -> torch.Tensor:

@@ -107,13 +107,19 @@ __device__ __forceinline__ uint32_t seen_keys(const AttendArgs &a, int32_t p_lo,
 __device__ __forceinline__ f32x16_p mfma(u32x4 x, u32x4 y, f32x16_p c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_p, x), __builtin_bit_cast(bf16x8_p, y), c, 0, 0, 0);
 }
-// Eight codes as bf16 numbers 128 + code: 0x4300 is 128 with seven fraction bits, the last four of which are the code.
-__device__ __forceinline__ u32x4 codes_to_bf16(uint32_t w) {
-    u32x4 r;
+// Eight codes as bf16 numbers 128 + code: 0x4300 is 128 with seven fraction bits, the last four of which are the code.  The
+// mask is kept in a vector register: with two constants the and-or would be two instructions (and three a pair, shift
+// included, instead of two).
+struct CodeMask {
+    uint32_t low_nibbles = 0x000F000Fu;
+    __device__ __forceinline__ CodeMask() { asm volatile("" : "+v"(low_nibbles)); }
+    __device__ __forceinline__ u32x4 to_bf16(uint32_t w) const {
+        u32x4 r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = (w >> (4 * j) & 0x000F000Fu) | 0x43004300u;
-    return r;
-}
+        for (int j = 0; j < 4; ++j) r[j] = (w >> (4 * j) & low_nibbles) | 0x43004300u;
+        return r;
+    }
+};
 __device__ __forceinline__ f32x16_p splat16(float x) {
     f32x16_p r;
 #pragma unroll
@@ -389,7 +395,6 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
     const int32_t pos = s.len - s.n + (int32_t)token_of(a, r0 + row);
     Running<D> run;
     run.clear();
-    const f32x16_p start = splat16(KIND == CI_KV_BF16 ? 0.0f : -128.0f * q.sum);
     const uint32_t last = min(u1 * kUnit, span.nb);
     bool lost = false;
 
@@ -411,42 +416,57 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
         return block_at<KIND, D>(a.cache, page == kNoPage ? 0 : page, it.head, blk);
     };
 
-    // keys are asked for one step ahead, values at the head of their step: a wavefront always has half a block on its way
-    Data x;
+    // bf16: a block's keys are asked for a step ahead and its values at the head of its own step (8 KB or more are then always on
+    // their way).  4 bits: a block is a quarter of that, so the next one is asked for whole, with its (step, low) pairs,
+    // before this one is begun (48 chats of up to 32 k tokens: 214 us as for bf16, 195 so; two blocks at a time 205).
+    constexpr bool kPairsAhead = NV <= 8;  // (registers do not go further)
+    const CodeMask codes;
+    Data x, y;
+    uint32_t kp[NV], vp[NV], kn[NV], vn[NV];
+    auto fetch_pairs = [&](const uint8_t *b, uint32_t (&kw)[NV], uint32_t (&vw)[NV]) {
+        const uint32_t *pairs = reinterpret_cast<const uint32_t *>(b + KvBlock<KIND, D>::kPairs);
+        cols.pairs(pairs, kw);
+        cols.pairs(pairs + kKvBlock, vw);
+    };
+    auto fetch_all = [&](const uint8_t *b, Data &d, uint32_t (&kw)[NV], uint32_t (&vw)[NV]) {
+        fetch_k(b, d);
+        fetch_v(b, d);
+        if (kPairsAhead) fetch_pairs(b, kw, vw);
+    };
     uint32_t i = u0 * kUnit + wave;
     const uint8_t *b = nullptr;
     if (i < last) {
         b = place(i);
-        fetch_k(b, x);
+        if (KIND == CI_KV_BF16) fetch_k(b, x);
+        else fetch_all(b, x, kp, vp);
     }
     for (; i < last; i += kUnit) {
         const int32_t kb = (int32_t)(span.block(i) * kKvBlock);
-        fetch_v(b, x);
         const bool edge = !all_visible(a, span, kb);
         uint32_t sees = 0xFFFFFFFFu;  // the lane's keys that its row sees, key0 as bit 0
         if (edge) sees = seen_keys(a, pos, pos, kb) >> cols.key0;
-        f32x16_p acc = start;
         if (KIND == CI_KV_BF16) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) acc = mfma(x.k[k], q.f[k], acc);
+            fetch_v(b, x);
         } else {
+            if (!kPairsAhead) fetch_pairs(b, kp, vp);
+            b = place(min(i + kUnit, last - 1));
+            fetch_all(b, y, kn, vn);
+        }
+        f32x16_p acc = splat16(0.0f);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) acc = mfma(codes_to_bf16(x.k[k / 4][k % 4]), q.f[k], acc);
+        for (int k = 0; k < D / 16; ++k)
+            acc = mfma(KIND == CI_KV_BF16 ? x.k[k % Data::N] : codes.to_bf16(x.k[k / 4 % Data::N][k % 4]), q.f[k], acc);
+        if (KIND == CI_KV_BF16) {
+            b = place(min(i + kUnit, last - 1));
+            fetch_k(b, x);
         }
-        uint32_t kp[NV], vp[NV];
-        if (KIND != CI_KV_BF16) {
-            const uint32_t *pairs = reinterpret_cast<const uint32_t *>(b + KvBlock<KIND, D>::kPairs);
-            cols.pairs(pairs, kp);
-            cols.pairs(pairs + kKvBlock, vp);
-        }
-        b = place(min(i + kUnit, last - 1));
-        fetch_k(b, x);
         float t[NV];
         cols.take(acc, t);
         float best = kNone;
 #pragma unroll
         for (int e = 0; e < NV; ++e) {
-            if (KIND != CI_KV_BF16) t[e] = t[e] * bf16_lo(kp[e]) + q.sum * bf16_hi(kp[e]);
+            // (q . (low + step code) from q . (128 + code))
+            if (KIND != CI_KV_BF16) t[e] = (t[e] - 128.0f * q.sum) * bf16_lo(kp[e]) + q.sum * bf16_hi(kp[e]);
             t[e] *= a.scale_log2;
             if (edge) t[e] = sees >> ((e & 3) + 8 * (e >> 2)) & 1 ? t[e] : kNone;
             best = most(best, t[e]);
@@ -456,7 +476,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
         uint32_t pk[NV / 2];
 #pragma unroll
         for (int e = 0; e < NV; e += 2) {
-            float p0 = exp2_fast(t[e] - base), p1 = exp2_fast(t[e + 1] - base);
+            const float p0 = exp2_fast(t[e] - base), p1 = exp2_fast(t[e + 1] - base);
             run.l += p0 + p1;
             if (KIND == CI_KV_BF16) {
                 pk[e / 2] = bf16_pair(p0, p1);
@@ -487,8 +507,15 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
 #pragma unroll
             for (int db = 0; db < D / 32; ++db) {
                 const int k = s2 * (D / 32) + db;
-                run.o[db] = mfma(KIND == CI_KV_BF16 ? x.v[k % Data::N] : codes_to_bf16(x.v[k / 4][k % 4]), f[s2], run.o[db]);
+                run.o[db] = mfma(KIND == CI_KV_BF16 ? x.v[k % Data::N] : codes.to_bf16(x.v[k / 4 % Data::N][k % 4]), f[s2], run.o[db]);
             }
+        if (KIND != CI_KV_BF16) {
+            x = y;
+            if (kPairsAhead) {
+#pragma unroll
+                for (int e = 0; e < NV; ++e) kp[e] = kn[e], vp[e] = vn[e];
+            }
+        }
     }
     if (lost) {
         if (lane == 0) report_bad_index(a.batch);
@@ -1264,7 +1291,10 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     uint64_t keys = longest;
     if (window && (uint64_t)window + sinks + 64 < keys) keys = (uint64_t)window + sinks + 64;
     p->whole = keys <= 4 * kUnit * kKvBlock;
-    p->workers = 2 * cus;
+    // as many as are resident; for 4 bits, where a workgroup waits longer for its first block than it then reads, twice as many
+    // if each still has much to do (48 chats of up to 32 k tokens 195 -> 187 us; one document of 65 k would lose, 28 -> 36)
+    const uint64_t units = (uint64_t)b.seqs * v.kv_heads * (keys / (kUnit * kKvBlock));
+    p->workers = (kind != CI_KV_BF16 && units >= 64ull * cus ? 4 : 2) * cus;
     p->grid = p->whole ? p->items : p->workers;
     if (!p->whole) p->work_bytes = (size_t)p->workers * 2 * p->rp * (head_dim + 2) * sizeof(float);
     return CI_OK;
