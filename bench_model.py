@@ -6,6 +6,7 @@ kernels' own contraction order applied to the plain weights (`plain_linear_same_
 whose generated ids the compressed model must reproduce exactly.
 
   python bench_model.py [--layers 32] [--prompt 128] [--new 256] [--tile-k 1024] [--gen cpu|cuda]
+                        [--kv-cache static|paged|paged-int4]
 
 Prints one JSON object: tokens per second of the compressed model (eager launches and one HIP
 graph replay per token), of the bf16 reference, and how the generated ids and logits compare.
@@ -14,7 +15,9 @@ Shape: hidden 4096, FFN 14336 SwiGLU, 32 query / 8 KV heads of 128, vocabulary 1
 RoPE theta 500000.  Weights bf16 N(0, 0.02) from seed 5 in module order (embedding; per layer q, k, v,
 o, gate, up, down; lm_head), norm weights 1; q/k/v and gate/up are compressed as fused projections
 (comp_inference/comp_inference.py:242-341).  Prompt: uniform random ids from seed 6.
-Everything except the linear / embedding / head operators is the same torch code in both models.
+Everything except the linear / embedding / head operators is the same in both models: torch code with a static
+cache (`--kv-cache static`, the default), or the package's paged cache in bf16 or 4 bits, with the rotation on
+the way in and its attention.
 """
 from __future__ import annotations
 
@@ -83,11 +86,21 @@ class PlainSameOrder:
 
 class Decoder:
     """The decoder over a set of operators: embed(ids) -> [T, H]; per layer qkv, o, gate_up, down;
-    head(x) -> [T, V].  Static KV cache so that one decode step has fixed shapes."""
+    head(x) -> [T, V].  The KV cache has a fixed size so that one decode step has fixed shapes: `kv` "static" (torch
+    tensors and torch's attention), or "paged" / "paged-int4" (PagedKVCache, paged_kv_append, paged_attention)."""
 
-    def __init__(self, ops, n_layers, max_len, dev):
+    def __init__(self, ops, n_layers, max_len, dev, kv="static"):
         s = Shape
-        self.ops, self.L, self.max_len, self.dev = ops, n_layers, max_len, dev
+        self.ops, self.L, self.max_len, self.dev, self.kv = ops, n_layers, max_len, dev, kv
+        if kv != "static":
+            import comp_inference_amd as ci
+
+            pages = -(-max_len // 64)
+            self.caches = [ci.PagedKVCache(pages, 64, s.kv_heads, s.head_dim, kind="int4" if kv == "paged-int4" else "bf16",
+                                           device=dev) for _ in range(n_layers)]
+            self.table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+            self.rotary = ci.rotary_table(max_len, s.head_dim, theta=s.theta, device=dev)
+            return
         self.k = torch.zeros(n_layers, s.kv_heads, max_len, s.head_dim, dtype=torch.bfloat16, device=dev)
         self.v = torch.zeros_like(self.k)
         inv = 1.0 / (s.theta ** (torch.arange(0, s.head_dim, 2, dtype=torch.float32, device=dev) / s.head_dim))
@@ -96,18 +109,32 @@ class Decoder:
         self.sin = torch.cat((ang.sin(), ang.sin()), dim=-1)
         self.positions = torch.arange(max_len, device=dev)
 
-    def _layer(self, l, h, pos, T):
-        """h [T, H]; pos int64 [T] (device).  Attention reads the whole cache, masked by position."""
+    def _paged_context(self, l, qkv, lens, start, T):
+        import comp_inference_amd as ci
+
+        s = Shape
+        q, k, v = qkv.split((s.heads, s.kv_heads, s.kv_heads), 1)
+        q = ci.paged_kv_append(self.caches[l], k, v, self.table, lens, start, q=q, rotary=self.rotary)
+        return ci.paged_attention(q, self.caches[l], self.table, lens, start, max_query_len=T, max_seq_len=self.max_len)
+
+    def _layer(self, l, h, pos, T, lens=None, start=None):
+        """h [T, H]; pos int64 [T] (device).  Static cache: attention reads the whole cache, masked by position."""
         s = Shape
         qkv = self.ops["qkv"][l](rmsnorm(h, s.eps))
         qkv = qkv.view(T, s.heads + 2 * s.kv_heads, s.head_dim)
+        if self.kv != "static":
+            return self._rest(l, h, self._paged_context(l, qkv, lens, start, T).reshape(T, s.heads * s.head_dim))
         qk = rope(qkv[:, :s.heads + s.kv_heads], self.cos.index_select(0, pos), self.sin.index_select(0, pos))
         self.k[l].index_copy_(1, pos, qk[:, s.heads:].transpose(0, 1))
         self.v[l].index_copy_(1, pos, qkv[:, s.heads + s.kv_heads:].transpose(0, 1))
         allowed = self.positions[None, :] <= pos[:, None]                        # [T, max_len]
         ctx = F.scaled_dot_product_attention(qk[:, :s.heads].transpose(0, 1)[None], self.k[l][None], self.v[l][None],
                                              attn_mask=allowed[None, None], enable_gqa=True)[0]  # [heads, T, d]
-        h = h + self.ops["o"][l](ctx.transpose(0, 1).reshape(T, s.heads * s.head_dim))
+        return self._rest(l, h, ctx.transpose(0, 1).reshape(T, s.heads * s.head_dim))
+
+    def _rest(self, l, h, ctx):
+        s = Shape
+        h = h + self.ops["o"][l](ctx)
         gu = self.ops["gate_up"][l](rmsnorm(h, s.eps))
         gate, up = gu.split((s.ffn, s.ffn), dim=-1)
         return h + self.ops["down"][l](F.silu(gate) * up)
@@ -116,8 +143,12 @@ class Decoder:
         """ids, pos int64 [T] -> logits of the last position [V] (fp32)."""
         T = ids.shape[0]
         h = self.ops["embed"](ids)
+        lens = start = None
+        if self.kv != "static":
+            lens = (pos[-1:] + 1).to(torch.int32)
+            start = None if T == 1 else torch.tensor([0, T], dtype=torch.int32).to(self.dev)
         for l in range(self.L):
-            h = self._layer(l, h, pos, T)
+            h = self._layer(l, h, pos, T, lens, start)
         return self.ops["head"](rmsnorm(h[-1:], Shape.eps)).float().view(-1)
 
 
@@ -251,7 +282,7 @@ def build(n_layers, dev, tile_k, tile_n, gen):
     return comp, ref, same, sizes
 
 
-def run(n_layers=32, n_prompt=128, n_new=256, tile_k=1024, tile_n=32, gen="cpu"):
+def run(n_layers=32, n_prompt=128, n_new=256, tile_k=1024, tile_n=32, gen="cpu", kv="static"):
     import comp_inference_amd as ci  # noqa: F401
 
     dev = torch.device("cuda", 0)
@@ -266,7 +297,7 @@ def run(n_layers=32, n_prompt=128, n_new=256, tile_k=1024, tile_n=32, gen="cpu")
                                  ("compressed_eager", comp, False), ("compressed_graph", comp, True),
                                  ("decompressed_same_order", same, False)):
             log(f"decoding: {name} ...")
-            dec = Decoder(ops, n_layers, max_len, dev)
+            dec = Decoder(ops, n_layers, max_len, dev, kv)
             ids, sec = generate(dec, prompt, n_new, graph)
             res[name] = (ids, sec)
             del dec
@@ -280,9 +311,9 @@ def run(n_layers=32, n_prompt=128, n_new=256, tile_k=1024, tile_n=32, gen="cpu")
     base = res["reference_bf16"][0]
     with torch.no_grad():
         log("teacher-forced comparison ...")
-        lr = teacher_forced(Decoder(ref, n_layers, max_len, dev), prompt, base)
-        lc = teacher_forced(Decoder(comp, n_layers, max_len, dev), prompt, base)
-        ls = teacher_forced(Decoder(same, n_layers, max_len, dev), prompt, base)
+        lr = teacher_forced(Decoder(ref, n_layers, max_len, dev, kv), prompt, base)
+        lc = teacher_forced(Decoder(comp, n_layers, max_len, dev, kv), prompt, base)
+        ls = teacher_forced(Decoder(same, n_layers, max_len, dev, kv), prompt, base)
     logits_bit_identical = bool(torch.equal(lc, ls))
     del ls
     forced_same = int((lr.argmax(-1) == lc.argmax(-1)).sum())
@@ -300,7 +331,7 @@ def run(n_layers=32, n_prompt=128, n_new=256, tile_k=1024, tile_n=32, gen="cpu")
 
     return {
         "model": f"Llama-3-8B shape, {n_layers} layers, random init seed 5 ({gen} generator), tile {tile_k}x{tile_n}",
-        "prompt_tokens": n_prompt, "new_tokens": n_new,
+        "prompt_tokens": n_prompt, "new_tokens": n_new, "kv_cache": kv,
         "weight_bytes_compressed": sizes["compressed"], "weight_bytes_bf16": sizes["bf16"],
         "checkpoint_index_bytes": int(index_bytes),
         "tok_per_s_compressed_graph": round(n_new / res["compressed_graph"][1], 2),
@@ -331,12 +362,13 @@ def main():
     ap.add_argument("--prompt", type=int, default=128)
     ap.add_argument("--new", type=int, default=256)
     ap.add_argument("--tile-k", type=int, default=1024)
+    ap.add_argument("--kv-cache", choices=("static", "paged", "paged-int4"), default="static")
     ap.add_argument("--gen", choices=("cpu", "cuda"), default="cpu")
     a = ap.parse_args()
     if not torch.cuda.is_available():
         print("bench_model.py needs a GPU (gfx950)", file=sys.stderr)
         return 2
-    print(json.dumps(run(a.layers, a.prompt, a.new, a.tile_k, 32, a.gen)))
+    print(json.dumps(run(a.layers, a.prompt, a.new, a.tile_k, 32, a.gen, a.kv_cache)))
     return 0
 
 

@@ -20,11 +20,11 @@ namespace ci {
 // values; code = (x - low) / step rounded to the nearest, ties to even.  Rows that hold an infinity or a NaN get
 // low = step = NaN and read back as NaN throughout.
 __device__ __forceinline__ uint32_t step_and_low(float low, float high) {
-    const double width = ((double)high - (double)low) / 15.0;
-    if (!(width < 3.0e38)) return 0x7FC07FC0u;  // NaN, infinite or beyond bf16
-    float f = (float)width;
-    if ((double)f < width) f = __uint_as_float(__float_as_uint(f) + 1);  // (width >= 0: the next float up)
-    const uint32_t step = (__float_as_uint(f) + 0xFFFFu) >> 16;
+    const double width = (double)high - (double)low;
+    // the least bf16 number whose fifteenfold (exact here) is not below the width: the quotient's neighbour, put right
+    uint32_t step = (__float_as_uint((float)(width * (1.0 / 15.0))) + 0xFFFFu) >> 16;
+    if (step && 15.0 * (double)bf16_lo(step - 1) >= width) --step;
+    if (15.0 * (double)bf16_lo(step) < width) ++step;
     return step | (__float_as_uint(low) & 0xFFFF0000u);  // (low is one of the row's bf16 values)
 }
 
@@ -47,8 +47,9 @@ __device__ __forceinline__ uint32_t code_of(float x, const Grid &g) {
     float t = (x - g.low) * g.inverse;
     if (g.extreme) t = (float)(((double)x - (double)g.low) / (double)g.step);
     float c = rintf(t);
-    // the float quotient is within a few units of 2^-20 of the exact one: only next to a border can it round wrongly
-    if (fabsf(fabsf(t - c) - 0.5f) < 1e-4f) {
+    // the float quotient, up to 15, is off by at most three roundings (3 x 15 x 2^-24 < 3e-6): only that near to a border can
+    // it round wrongly
+    if (fabsf(fabsf(t - c) - 0.5f) < 4e-6f || g.extreme) {
         const double r = ((double)x - (double)g.low) - (double)c * (double)g.step, half = 0.5 * (double)g.step;
         const bool odd = ((int)c & 1) != 0;
         if (r > half || (r == half && odd)) c += 1.0f;
@@ -168,19 +169,29 @@ __device__ __forceinline__ uint32_t codes8(u32x4 x, const Grid &g) {
     return word;
 }
 
-// min and max over the D / 16 neighbouring threads that share a row; (step, low) of the row.
+// The value of a neighbour in a row's threads: the other of a pair, of two pairs in four, of two fours in eight (in
+// which, by then, all of a four hold the same).
+template <int CTRL>
+__device__ __forceinline__ float neighbour(float x) {
+    const int v = __float_as_int(x);
+    return __int_as_float(__builtin_amdgcn_update_dpp(v, v, CTRL, 15, 15, false));
+}
+
+// min and max over the D / 16 neighbouring threads that share a row; (step, low) of the row.  Both carry a NaN (an infinity is
+// made one).
 template <int D>
 __device__ __forceinline__ uint32_t row_pair(u32x4 a, u32x4 b) {
-    float lo = fminf(min8(a), min8(b)), hi = fmaxf(max8(a), max8(b));
-    int wild = wild8(a) || wild8(b);
-#pragma unroll
-    for (int d = 1; d < D / 16; d *= 2) {
-        const int peer = (int)(threadIdx.x & 63) ^ d;
-        lo = fminf(lo, __int_as_float(__shfl(__float_as_int(lo), peer, 64)));
-        hi = fmaxf(hi, __int_as_float(__shfl(__float_as_int(hi), peer, 64)));
-        wild |= __shfl(wild, peer, 64);
+    const float wild = wild8(a) || wild8(b) ? __builtin_nanf("") : 0.0f;
+    float lo = fminf(min8(a), min8(b)) + wild, hi = fmaxf(max8(a), max8(b)) + wild;
+    lo = __builtin_elementwise_minimum(lo, neighbour<0xB1>(lo));
+    hi = __builtin_elementwise_maximum(hi, neighbour<0xB1>(hi));
+    lo = __builtin_elementwise_minimum(lo, neighbour<0x4E>(lo));
+    hi = __builtin_elementwise_maximum(hi, neighbour<0x4E>(hi));
+    if (D == 128) {
+        lo = __builtin_elementwise_minimum(lo, neighbour<0x141>(lo));
+        hi = __builtin_elementwise_maximum(hi, neighbour<0x141>(hi));
     }
-    return wild ? 0x7FC07FC0u : step_and_low(lo, hi);
+    return lo != lo ? 0x7FC07FC0u : step_and_low(lo, hi);
 }
 
 template <int KIND, int D>
