@@ -481,10 +481,12 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             if (KIND == CI_KV_BF16) {
                 pk[e / 2] = bf16_pair(p0, p1);
             } else {
-                // o = sum p (low + step code): the step goes into the weight, the low and the 128 of the code into `off`;
-                // a key that is not seen weighs nothing, whatever its step and low are
+                // o = sum p (low + step code): the step goes into the weight r = p step, which is rounded, and what is added back
+                // in 32 bits is sum p (low + 7.5 step) - sum r 135.5, so that the rounding of r meets code - 7.5 (as large as
+                // the value is away from its row's middle) and not the code, or 128 with it.  A key that is not seen weighs
+                // nothing, whatever its step and low are
                 const float s0 = p0 * bf16_lo(vp[e]), s1 = p1 * bf16_lo(vp[e + 1]);
-                float l0 = p0 * bf16_hi(vp[e]), l1 = p1 * bf16_hi(vp[e + 1]);
+                float l0 = fmaf(s0, 7.5f, p0 * bf16_hi(vp[e])), l1 = fmaf(s1, 7.5f, p1 * bf16_hi(vp[e + 1]));
                 pk[e / 2] = bf16_pair(s0, s1);
                 if (edge) {
                     const bool z0 = t[e] == kNone, z1 = t[e + 1] == kNone;
@@ -492,7 +494,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
                     l1 = z1 ? 0.0f : l1;
                     pk[e / 2] &= (z0 ? 0u : 0xFFFFu) | (z1 ? 0u : 0xFFFF0000u);
                 }
-                run.off += l0 + l1 - 128.0f * (bf16_lo(pk[e / 2]) + bf16_hi(pk[e / 2]));
+                run.off += l0 + l1 - 135.5f * (bf16_lo(pk[e / 2]) + bf16_hi(pk[e / 2]));
             }
         }
         u32x4 f[2];
@@ -752,7 +754,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
 // ---- many rows ------------------------------------------------------------------------------------------------------
 constexpr uint32_t kStep = 64;  // keys
 constexpr uint32_t kRowWaves = 8, kRowThreads = 64 * kRowWaves, kTileRows = 32 * kRowWaves;
-constexpr uint32_t rows_lds(int D) { return 2 * 2 * 128 * D; }  // two buffers of two blocks, keys and values in bf16
+constexpr uint32_t rows_lds(uint32_t kind, uint32_t D) {  // two buffers of two blocks, keys and values in bf16; steps and lows
+    return 2 * 2 * 128 * D + (kind == CI_KV_BF16 ? 0 : 4 * 128 * 4);
+}
 // Workgroups resident on a CU: registers allow two wavefronts per SIMD, four for heads of 64 in bf16.
 constexpr uint32_t row_groups(uint32_t kind, uint32_t dim) { return kind == CI_KV_BF16 && dim == 64 ? 2 : 1; }
 constexpr uint32_t kWholeSteps = 32;                             // a tile of up to so many steps is never cut
@@ -791,15 +795,16 @@ struct Stage<CI_KV_BF16, D> {
             if (is_value(i)) x[i] = keep_seen(x[i], (i < N / 2 ? held0 : held1) >> (16 * ((piece(i) - 4 * D) / (2 * D)) + 4 * h), 0);
     }
     // keys to buffer `kb`, values to buffer `vb`
-    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb) const {
+    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb, float *) const {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             reinterpret_cast<u32x4 *>((is_value(i) ? vb : kb) + (i < N / 2 ? 0 : 128 * D))[piece(i)] = x[i];
     }
 };
 
-// 4 bits: the codes become the values they stand for, rounded to bf16 (what a bf16 cache would hold of them), once for the
-// wavefronts that use them.  A wavefront takes a whole 1 KB piece of codes, keys or values of one block (for heads of 64
+// 4 bits: done once for the wavefronts that use them.  Keys become 128 + code, exact in bf16, and go with (step, low - 128 step)
+// of every key, which are applied to the scores in 32 bits: a key's own rounding to bf16 would be seen in its weight.  Values
+// become what they stand for, rounded to bf16 as a bf16 cache would hold them: that is averaged over the keys.  A wavefront takes a whole 1 KB piece of codes, keys or values of one block (for heads of 64
 // there are four pieces, and the second group has none).
 template <int D>
 struct Stage<CI_KV_INT4, D> {
@@ -846,19 +851,26 @@ struct Stage<CI_KV_INT4, D> {
         }
         return r;
     }
-    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb) const {
+    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb, float *key_pairs) const {
         if (N == 1 && idle()) return;
-        u32x4 *dst = reinterpret_cast<u32x4 *>((values() ? vb : kb) + block() * 128 * D + values() * 64 * D) + index() * 256 + (threadIdx.x & 63);
-        const uint32_t mask = 0u - values();  // (keys and values by the same instructions: a branch would stop the matrix unit)
+        const uint32_t lane = threadIdx.x & 63;
+        u32x4 *dst = reinterpret_cast<u32x4 *>((values() ? vb : kb) + block() * 128 * D + values() * 64 * D) + index() * 256 + lane;
+        const CodeMask codes;
+        const uint32_t val = 0u - values();  // (keys and values by the same instructions: a branch would stop the matrix unit)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             float step[8], low[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t w = (pair[(N == 2 ? 0 : c / 2 * 8) + e] & mask) | (own & ~mask);
+                const uint32_t w = pair[(N == 2 ? 0 : c / 2 * 8) + e];
                 step[e] = bf16_lo(w), low[e] = bf16_hi(w);
             }
-            dst[c * 64] = eight(x[c], step, low);
+            dst[c * 64] = (eight(x[c], step, low) & val) | (codes.to_bf16(x[c]) & ~val);
+        }
+        float *mine = key_pairs + block() * 32 + lane;
+        if (!values() && index() == 0 && lane < 32) {
+            mine[0] = bf16_lo(own);
+            mine[64] = fmaf(bf16_lo(own), -128.0f, bf16_hi(own));
         }
     }
 };
@@ -981,6 +993,9 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
     bool lost = false;  // whether a block was on no page of the cache (page 0 then stands for it, and the rows are done again)
     const uint32_t last_block = s.len > 0 ? (uint32_t)(s.len - 1) / kKvBlock : 0;
     const auto buffer = [&](uint32_t st) { return lds + (st & 1) * (256 * D); };
+    // 4 bits: step and low - 128 step of a step's keys, read in its vector phase (the second group's is phase 2 t + 2, in which
+    // the first stores those of step t + 2): four of them in turn
+    const auto key_pairs = [&](uint32_t st) { return reinterpret_cast<float *>(lds + 512 * D) + (st & 3) * 128; };
     const auto first_block = [&](uint32_t st) { return (uint32_t)steps.first_key(min(st, last - 1)) / kKvBlock; };
     const auto at_block = [&](uint32_t blk) {
         const uint32_t x = table.page_of(a.cache, blk);
@@ -996,7 +1011,7 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         stage.fetch(kp, vp);
     };
     // what is staged: keys of step ks, values of the step before
-    const auto put = [&](uint32_t ks) { stage.store(buffer(ks), buffer(ks - 1)); };
+    const auto put = [&](uint32_t ks) { stage.store(buffer(ks), buffer(ks - 1), key_pairs(ks)); };
     const auto clear = [&](uint32_t ks) {
         const int32_t kb = (int32_t)(first_block(ks - 1) * kKvBlock);
         if (kb + (int32_t)kStep > s.len) stage.clear(bits(0, s.len - kb), bits(0, s.len - kb - 32));
@@ -1048,6 +1063,18 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         // ---- vector phase
         hold(st + 3);
         clear(st + 2);
+        if (KIND != CI_KV_BF16) {  // q . (low + step code) from q . (128 + code)
+            const f32x4_p *of = reinterpret_cast<const f32x4_p *>(key_pairs(st));
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4_p s0 = of[2 * g + h], s1 = of[8 + 2 * g + h], l0 = of[16 + 2 * g + h], l1 = of[24 + 2 * g + h];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    acc0[4 * g + c] = fmaf(acc0[4 * g + c], s0[c], q.sum * l0[c]);
+                    acc1[4 * g + c] = fmaf(acc1[4 * g + c], s1[c], q.sum * l1[c]);
+                }
+            }
+        }
         if (st < clean0 || st >= clean1) {
             const int32_t kb = steps.first_key(st);
             const uint32_t s0 = seen_keys(a, pos, pos, kb) >> (4 * h), s1 = seen_keys(a, pos, pos, kb + 32) >> (4 * h);
@@ -1316,7 +1343,7 @@ template <int KIND, int D>
 static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
     if (p.many) {
         CI_ALLOW_FULL_LDS((attend_rows_kernel<KIND, D>));
-        CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(kRowThreads), rows_lds(D), s, a);
+        CI_KV_LAUNCH((attend_rows_kernel<KIND, D>), dim3(p.grid), dim3(kRowThreads), rows_lds(KIND, D), s, a);
         CI_LAUNCH_CHECK("attend_rows_kernel");
         if (!p.whole && p.workers > 1) {
             CI_KV_LAUNCH((attend_rows_join_kernel<KIND, D>), dim3(p.workers - 1, kTileRows / 32), dim3(256), 0, s, a, p.workers);
