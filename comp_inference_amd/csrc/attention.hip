@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
 constexpr uint32_t kStep = 64;  // keys
 constexpr uint32_t kRowWaves = 8, kRowThreads = 64 * kRowWaves, kTileRows = 32 * kRowWaves;
 constexpr uint32_t rows_lds(uint32_t kind, uint32_t D) {  // two buffers of two blocks, keys and values in bf16; steps and lows
-    return 2 * 2 * 128 * D + (kind == CI_KV_BF16 ? 0 : 4 * 128 * 4);
+    return 2 * 2 * 128 * D + (kind == CI_KV_BF16 ? 0 : 4 * 256 * 4);
 }
 // Workgroups resident on a CU: registers allow two wavefronts per SIMD, four for heads of 64 in bf16.
 constexpr uint32_t row_groups(uint32_t kind, uint32_t dim) { return kind == CI_KV_BF16 && dim == 64 ? 2 : 1; }
@@ -788,89 +788,69 @@ struct Stage<CI_KV_BF16, D> {
         }
     }
     // values of tokens that are not there become zero
-    __device__ __forceinline__ void clear(uint32_t held0, uint32_t held1) {
+    __device__ __forceinline__ void clear(uint32_t, uint32_t, uint32_t held0, uint32_t held1) {
         const uint32_t h = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (is_value(i)) x[i] = keep_seen(x[i], (i < N / 2 ? held0 : held1) >> (16 * ((piece(i) - 4 * D) / (2 * D)) + 4 * h), 0);
     }
     // keys to buffer `kb`, values to buffer `vb`
-    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb, float *) const {
+    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb, float *, float) const {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             reinterpret_cast<u32x4 *>((is_value(i) ? vb : kb) + (i < N / 2 ? 0 : 128 * D))[piece(i)] = x[i];
     }
 };
 
-// 4 bits: done once for the wavefronts that use them.  Keys become 128 + code, exact in bf16, and go with (step, low - 128 step)
-// of every key, which are applied to the scores in 32 bits: a key's own rounding to bf16 would be seen in its weight.  Values
-// become what they stand for, rounded to bf16 as a bf16 cache would hold them: that is averaged over the keys.  A wavefront takes a whole 1 KB piece of codes, keys or values of one block (for heads of 64
-// there are four pieces, and the second group has none).
+// 4 bits: codes become code - 7.5, exact in bf16, once for the wavefronts that use them; a key or value stands for
+// mid + step (code - 7.5), mid = low + 7.5 step.  Step and mid are applied in 32 bits: to the scores (keys; with the scale), and to
+// the weights before they are rounded (values), so what a 4-bit row stands for is never rounded itself, and a weight once,
+// as over a bf16 cache.  A wavefront takes a whole 1 KB piece of codes, keys or values of one block (for heads of 64 there are
+// four pieces, and the second group has none); the one with a block's first keys also takes the 64 (step, low) pairs.
 template <int D>
 struct Stage<CI_KV_INT4, D> {
     static constexpr int N = D / 64;  // pieces of the keys of a block
     u32x4 x;
-    uint32_t own, pair[16 / N];  // (step, low): of the lane's key; of its tokens in the values (16 for heads of 64, 8 for 128)
+    uint32_t pair;  // (step, low): of key `lane`, from lane 32 on of value lane - 32 of the step's keys' block
     static __device__ __forceinline__ uint32_t unit() { return uniform(threadIdx.x >> 6); }
     static __device__ __forceinline__ bool idle() { return unit() >= 4 * N; }
     static __device__ __forceinline__ uint32_t block() { return unit() / (2 * N) & 1; }
     static __device__ __forceinline__ uint32_t values() { return unit() / N & 1; }
     static __device__ __forceinline__ uint32_t index() { return unit() % N; }
     __device__ __forceinline__ void fetch(const Blocks &kb, const Blocks &vb) {
-        const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
+        const uint32_t lane = threadIdx.x & 63;
         // (chosen by arithmetic: a choice between the four would put them into memory)
         const int64_t blk = -(int64_t)block(), val = -(int64_t)values();
         const uint8_t *k = kb.b0 + ((kb.b1 - kb.b0) & blk), *v = vb.b0 + ((vb.b1 - vb.b0) & blk), *b = k + ((v - k) & val);
         x = reinterpret_cast<const u32x4 *>(b + values() * KvBlock<CI_KV_INT4, D>::kHalf)[index() * 64 + lane];
-        // tokens 16 s + 8 a + 4 h + b, s = the piece's index for heads of 128
-        const uint32_t *p = reinterpret_cast<const uint32_t *>(b + KvBlock<CI_KV_INT4, D>::kPairs);
-        own = p[lane & 31];
-#pragma unroll
-        for (uint32_t c = 0; c < 16 / N; c += 4) {
-            const uint32_t s = N == 2 ? index() : c / 8;
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(p + kKvBlock + 16 * s + 8 * (c / 4 % 2) + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) pair[c + e] = w[e];
-        }
+        pair = reinterpret_cast<const uint32_t *>(k + KvBlock<CI_KV_INT4, D>::kPairs)[lane];
     }
-    // (a value of a token that is not there: step 0, low 0)
-    __device__ __forceinline__ void clear(uint32_t held0, uint32_t held1) {
-        const uint32_t here = (block() ? held1 : held0) >> (4 * ((threadIdx.x >> 5) & 1) + (N == 2 ? 16 * index() : 0));
-#pragma unroll
-        for (uint32_t c = 0; c < 16 / N; ++c)
-            if (!(here >> (16 * (c / 8) + value_token(0, 0, c % 8)) & 1)) pair[c] = 0;
+    // (a value of a token that is not there: step 0, mid 0)
+    __device__ __forceinline__ void clear(uint32_t keys0, uint32_t keys1, uint32_t, uint32_t) {
+        const uint32_t lane = threadIdx.x & 63, held = block() ? keys1 : keys0;
+        if (lane >= 32 && !(held >> (lane & 31) & 1)) pair = 0;
     }
-    static __device__ __forceinline__ u32x4 eight(uint32_t word, const float (&step)[8], const float (&low)[8]) {
+    static __device__ __forceinline__ u32x4 centred(uint32_t word) {
         const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;  // codes 0, 4, 1, 5 and 2, 6, 3, 7, a byte each
         u32x4 r;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const uint32_t from = w % 2 ? odd : even;
-            const float c0 = (float)(from >> (w < 2 ? 0 : 8) & 0xFFu), c1 = (float)(from >> (w < 2 ? 16 : 24) & 0xFFu);
-            r[w] = bf16_pair(fmaf(step[2 * w], c0, low[2 * w]), fmaf(step[2 * w + 1], c1, low[2 * w + 1]));
+            r[w] = bf16_pair((float)(from >> (w < 2 ? 0 : 8) & 0xFFu) - 7.5f, (float)(from >> (w < 2 ? 16 : 24) & 0xFFu) - 7.5f);
         }
         return r;
     }
-    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb, float *key_pairs) const {
+    __device__ __forceinline__ void store(uint8_t *kb, uint8_t *vb, float *grid, float scale) const {
         if (N == 1 && idle()) return;
         const uint32_t lane = threadIdx.x & 63;
         u32x4 *dst = reinterpret_cast<u32x4 *>((values() ? vb : kb) + block() * 128 * D + values() * 64 * D) + index() * 256 + lane;
-        const CodeMask codes;
-        const uint32_t val = 0u - values();  // (keys and values by the same instructions: a branch would stop the matrix unit)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            float step[8], low[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t w = pair[(N == 2 ? 0 : c / 2 * 8) + e];
-                step[e] = bf16_lo(w), low[e] = bf16_hi(w);
-            }
-            dst[c * 64] = (eight(x[c], step, low) & val) | (codes.to_bf16(x[c]) & ~val);
-        }
-        float *mine = key_pairs + block() * 32 + lane;
-        if (!values() && index() == 0 && lane < 32) {
-            mine[0] = bf16_lo(own);
-            mine[64] = fmaf(bf16_lo(own), -128.0f, bf16_hi(own));
+        for (int c = 0; c < 4; ++c) dst[c * 64] = centred(x[c]);
+        if (!values() && index() == 0) {
+            const float f = lane < 32 ? scale : 1.0f, step = bf16_lo(pair) * f;
+            float *mine = grid + (lane >> 5) * 128 + block() * 32 + (lane & 31);
+            mine[0] = step;
+            mine[64] = fmaf(step, 7.5f, bf16_hi(pair) * f);
         }
     }
 };
@@ -993,9 +973,9 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
     bool lost = false;  // whether a block was on no page of the cache (page 0 then stands for it, and the rows are done again)
     const uint32_t last_block = s.len > 0 ? (uint32_t)(s.len - 1) / kKvBlock : 0;
     const auto buffer = [&](uint32_t st) { return lds + (st & 1) * (256 * D); };
-    // 4 bits: step and low - 128 step of a step's keys, read in its vector phase (the second group's is phase 2 t + 2, in which
-    // the first stores those of step t + 2): four of them in turn
-    const auto key_pairs = [&](uint32_t st) { return reinterpret_cast<float *>(lds + 512 * D) + (st & 3) * 128; };
+    // 4 bits: steps and mids of a step's keys and values, [2][step 64, mid 64], stored with its keys and read in its vector phase
+    // (the second group's is phase 2 t + 2, in which the first stores those of step t + 2): four of them in turn
+    const auto grid = [&](uint32_t st) { return reinterpret_cast<float *>(lds + 512 * D) + (st & 3) * 256; };
     const auto first_block = [&](uint32_t st) { return (uint32_t)steps.first_key(min(st, last - 1)) / kKvBlock; };
     const auto at_block = [&](uint32_t blk) {
         const uint32_t x = table.page_of(a.cache, blk);
@@ -1011,10 +991,11 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         stage.fetch(kp, vp);
     };
     // what is staged: keys of step ks, values of the step before
-    const auto put = [&](uint32_t ks) { stage.store(buffer(ks), buffer(ks - 1), key_pairs(ks)); };
+    const auto put = [&](uint32_t ks) { stage.store(buffer(ks), buffer(ks - 1), grid(ks), a.scale_log2); };
     const auto clear = [&](uint32_t ks) {
-        const int32_t kb = (int32_t)(first_block(ks - 1) * kKvBlock);
-        if (kb + (int32_t)kStep > s.len) stage.clear(bits(0, s.len - kb), bits(0, s.len - kb - 32));
+        const int32_t kb = (int32_t)(first_block(ks) * kKvBlock), vb = (int32_t)(first_block(ks - 1) * kKvBlock);
+        if (max(kb, vb) + (int32_t)kStep > s.len)
+            stage.clear(bits(0, s.len - kb), bits(0, s.len - kb - 32), bits(0, s.len - vb), bits(0, s.len - vb - 32));
     };
     const auto hold = [&](uint32_t st) { table.hold(a.batch, a.cache, first_block(st)); };
     // steps [clean0, clean1) need no mask for the wavefront's rows
@@ -1047,6 +1028,7 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         kp.b0 = at_block(first_block(u0));  // (the first step's values go with its keys, unread)
         kp.b1 = kp.b0;
         ask(u0);
+        clear(u0);
         put(u0);
         hold(u0 + 1);
         ask(u0 + 1);
@@ -1063,15 +1045,15 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         // ---- vector phase
         hold(st + 3);
         clear(st + 2);
-        if (KIND != CI_KV_BF16) {  // q . (low + step code) from q . (128 + code)
-            const f32x4_p *of = reinterpret_cast<const f32x4_p *>(key_pairs(st));
+        const f32x4_p *of = reinterpret_cast<const f32x4_p *>(grid(st)) + h;
+        if (KIND != CI_KV_BF16) {  // scale q . (mid + step (code - 7.5)), from q . (code - 7.5) and the sum of q
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4_p s0 = of[2 * g + h], s1 = of[8 + 2 * g + h], l0 = of[16 + 2 * g + h], l1 = of[24 + 2 * g + h];
+                const f32x4_p s0 = of[2 * g], s1 = of[8 + 2 * g], m0 = of[16 + 2 * g], m1 = of[24 + 2 * g];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    acc0[4 * g + c] = fmaf(acc0[4 * g + c], s0[c], q.sum * l0[c]);
-                    acc1[4 * g + c] = fmaf(acc1[4 * g + c], s1[c], q.sum * l1[c]);
+                    acc0[4 * g + c] = fmaf(acc0[4 * g + c], s0[c], q.sum * m0[c]);
+                    acc1[4 * g + c] = fmaf(acc1[4 * g + c], s1[c], q.sum * m1[c]);
                 }
             }
         }
@@ -1087,13 +1069,20 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         float best = kNone;
 #pragma unroll
         for (int e = 0; e < 16; ++e) best = most(best, most(acc0[e], acc1[e]));
-        run.raise(max_halves(best) * a.scale_log2);
+        const float scale = KIND == CI_KV_BF16 ? a.scale_log2 : 1.0f;
+        run.raise(max_halves(best) * scale);
         const float base = run.base();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-            const float x0 = exp2_fast(acc0[e] * a.scale_log2 - base), x1 = exp2_fast(acc0[e + 1] * a.scale_log2 - base);
-            const float y0 = exp2_fast(acc1[e] * a.scale_log2 - base), y1 = exp2_fast(acc1[e + 1] * a.scale_log2 - base);
+            float x0 = exp2_fast(acc0[e] * scale - base), x1 = exp2_fast(acc0[e + 1] * scale - base);
+            float y0 = exp2_fast(acc1[e] * scale - base), y1 = exp2_fast(acc1[e + 1] * scale - base);
             run.l += (x0 + x1) + (y0 + y1);
+            if (KIND != CI_KV_BF16) {  // sum w (mid + step (code - 7.5))
+                const int g = e / 4, c = e % 4;
+                const f32x4_p s0 = of[32 + 2 * g], s1 = of[40 + 2 * g], m0 = of[48 + 2 * g], m1 = of[56 + 2 * g];
+                run.off = fmaf(x0, m0[c], fmaf(x1, m0[c + 1], fmaf(y0, m1[c], fmaf(y1, m1[c + 1], run.off))));
+                x0 *= s0[c], x1 *= s0[c + 1], y0 *= s1[c], y1 *= s1[c + 1];
+            }
             p[e / 8][e / 2 % 4] = bf16_pair(x0, x1);
             p[2 + e / 8][e / 2 % 4] = bf16_pair(y0, y1);
         }
@@ -1118,6 +1107,13 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
     }
     const float l = run.l + other_half(run.l);
     const bool mine = r0 + col < t1;
+    if (KIND != CI_KV_BF16) {
+        const float off = run.off + other_half(run.off);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) run.o[db][k] += off;
+    }
     if (!whole) {
         if (!mine) return;
         float *o = slot + (r0 - t0 + col) * D;
