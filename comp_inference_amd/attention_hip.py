@@ -70,11 +70,11 @@ class PagedKVCache:
     def _struct(self):
         """The C descriptor by reference; made again when `data` is another memory."""
         d = self.data
-        at = d.data_ptr()
+        at = (d.data_ptr(), d.nbytes)
         if self._bound is None or self._bound[0] != at or not d.is_contiguous():
             if not d.is_contiguous():
                 raise RuntimeError("the cache's data must stay contiguous")
-            c = _Cache(at, d.numel() * d.element_size(), self.num_pages, self.page_size, self.kv_heads, self.head_dim,
+            c = _Cache(*at, self.num_pages, self.page_size, self.kv_heads, self.head_dim,
                        KINDS[self.kind])
             self._bound = (at, c, C.byref(c))
         return self._bound[2]
@@ -113,7 +113,7 @@ def _batch(cache: PagedKVCache, index: int, block_table, seq_lens, query_start, 
         start = query_start.data_ptr()
     if ok:
         (rows, width), (step, inner) = block_table.shape, block_table.stride()
-        if rows == seqs and (start is not None or tokens == seqs) and (inner == 1 or width <= 1) and step >= 0:
+        if rows == seqs and (start is not None or tokens == seqs) and (inner == 1 or width <= 1) and 0 <= step < 1 << 32:
             return C.byref(_Batch(block_table.data_ptr(), step if seqs > 1 else width, width, seq_lens.data_ptr(), start,
                                   seqs, tokens))
     for name, t, dim in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1), ("query_start", query_start, 1)):
@@ -166,7 +166,7 @@ def paged_kv_append(cache: PagedKVCache, k, v, block_table, seq_lens, query_star
     batch's new tokens: the last ones of every sequence.  With `rotary` (a table as `rotary_table` makes; channels d and
     d + rotary_dim / 2 form a pair, the channels behind rotary_dim stay) keys and queries are turned by their position's
     angle first; the rotation is exact up to its one rounding to bf16.  `q` [T, heads, head_dim] is turned the same way
-    into `q_out` (may be `q` itself; made if not given), which is returned.  Rows behind the last sequence, and
+    into `q_out` (`q` itself, or memory of its own; made if not given), which is returned.  Rows behind the last sequence, and
     sequences of length 0, are left as they were.  Tokens, pages and table rows that do not exist are left out and
     reported by `device_status`."""
     _lib.require_device(cache.data)
@@ -226,7 +226,8 @@ def paged_attention(q, cache: PagedKVCache, block_table, seq_lens, query_start=N
     """softmax(scale * q k^T) v over the visible keys of every query's sequence; q [T, heads, head_dim] in bf16, heads a
     multiple of the cache's kv heads.  The query at position p sees key j when j <= p and, with a `window` > 0, p - j <
     window or j < `sinks`.  A row that sees nothing (a sequence of length 0) gets zeros; rows behind the last sequence are
-    not written.  `scale`: 1 / sqrt(head_dim) if not given; positive.  `max_query_len`, `max_seq_len`: what the caller
+    not written.  With a window, pages that hold no key a new token sees need not be named in `block_table` (any entry
+    will do).  `out` shares no memory with q.  `scale`: 1 / sqrt(head_dim) if not given; positive.  `max_query_len`, `max_seq_len`: what the caller
     knows about the longest sequence (0: nothing); they choose kernels, the results do not rest on them.  `return_lse`:
     also fp32 [T, heads], the natural logarithm of the sum of exp(scores).  Scores, sums and the output are held in 32
     bits; the weights are rounded to bf16 for the product with v.  Inference only."""

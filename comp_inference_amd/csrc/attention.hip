@@ -997,7 +997,14 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         if (max(kb, vb) + (int32_t)kStep > s.len)
             stage.clear(bits(0, s.len - kb), bits(0, s.len - kb - 32), bits(0, s.len - vb), bits(0, s.len - vb - 32));
     };
-    const auto hold = [&](uint32_t st) { table.hold(a.batch, a.cache, first_block(st)); };
+    const auto hold = [&](uint32_t st) {
+        if (!table.hold(a.batch, a.cache, first_block(st)) || !a.window) return;
+        // a page of a step that lies before the window's first key and behind the sinks is seen by no row of the tile and may be
+        // gone: page 0 stands for it (looked at here, not where blocks are asked for: there it would stop the matrix unit,
+        // 777 instead of 552 us for a prompt of 8192 tokens)
+        const uint32_t at = table.held * 64 + lane, shift = a.cache.page_shift + 5;
+        if ((int32_t)((at + 1) << shift) <= position_of(a, s, t0) - a.window + 1 && at << shift >= (uint32_t)a.sinks) table.pages = 0;
+    };
     // steps [clean0, clean1) need no mask for the wavefront's rows
     const uint32_t clean0 = a.window ? steps.s1 + (p_hi - a.window < 0 ? 0u : max((uint32_t)(p_hi - a.window) / kStep + 1, steps.w0) - steps.w0) : 0;
     const uint32_t clean1 = p_lo + 1 < (int32_t)kStep ? 0 : steps.s1 + max((uint32_t)(p_lo + 1) / kStep, steps.w0) - steps.w0;
@@ -1299,6 +1306,10 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     const uint64_t items = tiles * v.kv_heads;
     if (items > 0x7FFFFF00ull) return fail(CI_ERR_ARG, "ci_paged_attention: too many rows for one call");
     p->items = (uint32_t)items;
+    // places in the list of work, at most (an item of few rows goes in units, a tile of many in steps): 32 bits count them
+    const uint64_t room = (uint64_t)b.table_width << (v.page_shift + 5);
+    if (room / (p->many ? kStep : kUnit * kKvBlock) + 2 > 0xFF000000ull / (items ? items : 1))
+        return fail(CI_ERR_ARG, "ci_paged_attention: too many rows over too long a block table for one call; give the rows in several");
     if (p->many) {
         p->workers = p->grid = (cus * row_groups(kind, head_dim) + 7) / 8 * 8;
         // tiles of few steps: one workgroup each, handed out by the hardware, and nothing to join (ragged prompts of up to 6001
@@ -1400,6 +1411,8 @@ extern "C" int ci_paged_attention(const ci_kv_cache *cache, const ci_kv_batch *b
             return fail(CI_ERR_ARG, "%s: %s must be a 16-byte aligned device pointer with strides that are non-negative multiples of 8",
                         who, r == q ? "q" : "out");
     }
+    if (rows_may_overlap(*q, q_heads, *out, q_heads, a.batch.tokens, cache->head_dim))  // (a row may be done a second time)
+        return fail(CI_ERR_ARG, "%s: out must share no memory with q", who);
     a.q = static_cast<const uint16_t *>(q->d_data);
     a.out = static_cast<uint16_t *>(out->d_data);
     a.lse = d_lse;

@@ -13,6 +13,8 @@
 // keep up with the memory here (a dozen 64-bit operations per 16 bytes).
 #include "paged.h"
 
+#include <numeric>
+
 namespace ci {
 
 // ---- what a row in 4 bits is ---------------------------------------------------------------------------------------
@@ -411,6 +413,26 @@ int check_kv_batch(const char *who, const ci_kv_batch *b, const KvView &v, KvBat
     return CI_OK;
 }
 
+// Whether two row tensors may share an element.  They share none if their extents are apart, if one's rows lie in the gaps
+// between the other's (slices of [tokens, heads, dim] along heads), or if the heads do (slices of [tokens, heads, 3, dim]).
+bool rows_may_overlap(const ci_rows &a, uint32_t a_heads, const ci_rows &b, uint32_t b_heads, uint32_t tokens, uint32_t dim) {
+    const auto width = [&](const ci_rows &r, uint32_t heads) { return (int64_t)(heads - 1) * r.head_stride + dim; };
+    const int64_t wa = width(a, a_heads), wb = width(b, b_heads), D = dim;
+    const int64_t off = ((intptr_t)b.d_data - (intptr_t)a.d_data) / 2;  // (both 16-byte aligned)
+    const int64_t rows = tokens - 1;
+    if (off >= rows * a.row_stride + wa || -off >= rows * b.row_stride + wb) return false;
+    const auto apart = [&](int64_t every, int64_t first, int64_t second) {  // [0, first) and off + [0, second), every so many
+        const int64_t at = every ? (off % every + every) % every : 0;
+        return every && at >= first && at + second <= every;
+    };
+    if (rows && a.row_stride == b.row_stride && apart(a.row_stride, wa, wb)) return false;
+    int64_t every = 0;
+    if (rows) every = std::gcd(a.row_stride, b.row_stride);
+    if (a_heads > 1) every = std::gcd(every, a.head_stride);
+    if (b_heads > 1) every = std::gcd(every, b.head_stride);
+    return !apart(every, D, D);
+}
+
 // Workgroups in x: the blocks of 32 that the new tokens of a batch can touch at most (a sequence with n of them touches at
 // most n, and at most n / 32 + 2).
 static uint32_t tile_bound(const KvBatch &b) {
@@ -459,6 +481,11 @@ extern "C" int ci_paged_kv_append(const ci_kv_cache *cache, const ci_kv_batch *b
     if (q) {
         if (int rc = check_rows(who, "q", q->d_data, q->row_stride, q->head_stride, q_heads)) return rc;
         if (int rc = check_rows(who, "q_out", q_out->d_data, q_out->row_stride, q_out->head_stride, q_heads)) return rc;
+        const bool same = q->d_data == q_out->d_data && q->row_stride == q_out->row_stride && q->head_stride == q_out->head_stride;
+        const uint32_t n = a.batch.tokens, dim = cache->head_dim, kv = a.cache.kv_heads;
+        if ((!same && rows_may_overlap(*q, q_heads, *q_out, q_heads, n, dim)) || rows_may_overlap(*k, kv, *q_out, q_heads, n, dim) ||
+            rows_may_overlap(*v, kv, *q_out, q_heads, n, dim))
+            return fail(CI_ERR_ARG, "%s: q_out must be q itself or share no memory with q, k and v", who);
         a.q = static_cast<const uint16_t *>(q->d_data);
         a.q_out = static_cast<uint16_t *>(q_out->d_data);
         a.q_row = q->row_stride, a.q_head = q->head_stride, a.o_row = q_out->row_stride, a.o_head = q_out->head_stride;
@@ -498,6 +525,8 @@ extern "C" int ci_paged_kv_read(const ci_kv_cache *cache, const ci_kv_batch *bat
     if (a.batch.seqs == 0 || a.batch.tokens == 0) return CI_OK;
     if (int rc = check_rows(who, "k", k->d_data, k->row_stride, k->head_stride, a.cache.kv_heads)) return rc;
     if (int rc = check_rows(who, "v", v->d_data, v->row_stride, v->head_stride, a.cache.kv_heads)) return rc;
+    if (rows_may_overlap(*k, a.cache.kv_heads, *v, a.cache.kv_heads, a.batch.tokens, cache->head_dim))
+        return fail(CI_ERR_ARG, "%s: k and v must not share memory", who);
     a.k = static_cast<uint16_t *>(k->d_data);
     a.v = static_cast<uint16_t *>(v->d_data);
     a.k_row = k->row_stride, a.k_head = k->head_stride, a.v_row = v->row_stride, a.v_head = v->head_stride;

@@ -118,14 +118,14 @@ struct PageRun {
     const int32_t *row;
     uint32_t held, pages;  // which 64 entries; this lane's
     __device__ __forceinline__ PageRun(const KvBatch &b, uint32_t seq) : row(b.table + (uint64_t)seq * b.table_stride), held(kNoPage), pages(0) {}
-    // makes sure that the entry of block `blk` is among those held
-    __device__ __forceinline__ void hold(const KvBatch &b, const KvView &v, uint32_t blk) {
+    // makes sure that the entry of block `blk` is among those held; whether they were loaded anew
+    __device__ __forceinline__ bool hold(const KvBatch &b, const KvView &v, uint32_t blk) {
         const uint32_t which = blk >> v.page_shift >> 6;
-        if (which != held) {
-            held = which;
-            const uint32_t at = held * 64 + (threadIdx.x & 63);
-            pages = at < b.table_width ? (uint32_t)row[at] : kNoPage;
-        }
+        if (which == held) return false;
+        held = which;
+        const uint32_t at = held * 64 + (threadIdx.x & 63);
+        pages = at < b.table_width ? (uint32_t)row[at] : kNoPage;
+        return true;
     }
     // the page of a block whose entry is held
     __device__ __forceinline__ uint32_t page_of(const KvView &v, uint32_t blk) const {
@@ -206,6 +206,7 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 // host side
 int check_kv_cache(const char *who, const ci_kv_cache *c, KvView *v);
 int check_kv_batch(const char *who, const ci_kv_batch *b, const KvView &v, KvBatch *out);
+bool rows_may_overlap(const ci_rows &a, uint32_t a_heads, const ci_rows &b, uint32_t b_heads, uint32_t tokens, uint32_t dim);
 
 #define CI_KV_LAUNCH(kernel, grid, block, shmem, stream, ...) hipLaunchKernelGGL(kernel, grid, block, shmem, stream, __VA_ARGS__)
 

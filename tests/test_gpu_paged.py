@@ -510,3 +510,24 @@ def test_what_a_row_does_not_see_may_be_anything(kind, lens, news, longest):
             assert not torch.isfinite(got[rows][sees][..., 2::4]).any()  # (the channels whose value is NaN)
             at += n
     assert ci.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int4"])
+@pytest.mark.parametrize("lens,news,longest", [([700], [300], 0), ([700, 1450], [300, 260], 0), ([410, 100], [3, 1], 3)])
+@pytest.mark.parametrize("window,sinks", [(50, 0), (50, 5), (97, 40), (20, 0)])
+def test_pages_before_the_window_may_be_gone(kind, lens, news, longest, window, sinks):
+    """Pages of 32 tokens that hold no key a new token sees are taken out of the table: the results stay, and nothing that
+    does not exist is reported."""
+    ci = _ci()
+    f = Filled(lens, news, 8, 2, 64, kind, page=32, seed=71)
+    kw = dict(window=window, sinks=sinks, max_query_len=longest)
+    whole = ci.paged_attention(f.q.to(DEV), *f.args(), **kw)
+    table = f.table.clone()
+    for b, (l, n) in enumerate(zip(lens, news)):
+        gone = torch.arange(table.shape[1]) * 32
+        gone = (gone >= sinks) & (gone + 31 < l - n - window + 1)
+        table[b, gone.to(DEV)] = -1
+        assert gone.any() or l == 100
+    got = ci.paged_attention(f.q.to(DEV), f.cache, table, f.seq, f.start, **kw)
+    assert torch.equal(got, whole)
+    assert ci.device_status() == 0

@@ -111,6 +111,57 @@ def test_arguments_of_each_entry_point(entry, field, value, code, said):
     assert said in lib.ci_last_error(), lib.ci_last_error()
 
 
+def _placed(at, row=1024, head=128):
+    from comp_inference_amd import attention_hip as A
+
+    return A._Rows(0x100000 + 2 * at, row, head)
+
+
+@pytest.mark.parametrize("entry,change,refused", [
+    ("attend", dict(q=_placed(0), out=_placed(0)), True),                         # in place
+    ("attend", dict(q=_placed(0), out=_placed(1024)), True),                      # a row further
+    ("attend", dict(q=_placed(9 * 1024), out=_placed(0)), True),                  # the last row
+    ("attend", dict(q=_placed(9 * 1024 + 512), out=_placed(0, 1024)), False),     # in the last row's gap
+    ("attend", dict(q=_placed(0), out=_placed(512)), False),                      # heads 4..7 of rows of eight
+    ("attend", dict(q=_placed(512), out=_placed(0)), False),
+    ("attend", dict(q=_placed(0), out=_placed(504)), True),
+    ("attend", dict(q=_placed(0, 1536, 384), out=_placed(128, 1536, 384)), False),  # [tokens, heads, 3, dim]
+    ("attend", dict(q=_placed(0, 1536, 384), out=_placed(8, 1536, 384)), True),
+    ("attend", dict(q=_placed(0, 128, 1280), out=_placed(5120, 128, 1280)), False),  # heads outermost, one after the other
+    ("attend", dict(q=_placed(0, 128, 1280), out=_placed(5112, 128, 1280)), True),
+    ("append", dict(q=_placed(0), out=_placed(8), k=_placed(1 << 20), v=_placed(2 << 20)), True),
+    ("append", dict(q=_placed(0), out=_placed(0, 1024, 136), k=_placed(1 << 20), v=_placed(2 << 20)), True),
+    ("append", dict(q=_placed(0), out=_placed(3 << 20), k=_placed(3 << 20), v=_placed(2 << 20)), True),
+    ("append", dict(q=_placed(0), out=_placed(3 << 20), k=_placed(1 << 20), v=_placed((3 << 20) + 384)), True),
+    ("append", dict(q=_placed(0), out=_placed(0), k=_placed(512), v=_placed(768)), False),  # one buffer, queries in place
+    ("read", dict(k=_placed(0), v=_placed(128)), True),
+    ("read", dict(k=_placed(0), v=_placed(256)), False)])
+def test_outputs_do_not_lie_on_other_operands(entry, change, refused):
+    """(What is let through ends a check later, for want of a device here or of a workspace: the pointers are never followed.)"""
+    from comp_inference_amd import _lib
+
+    if not refused and torch.cuda.is_available():
+        pytest.skip("a call that is not refused would run")
+    lib = _lib.lib()
+    a = _Args()
+    a.workspace = None
+    for name, rows in change.items():
+        setattr(a, name, rows)
+    assert getattr(a, entry)(lib) != 0
+    assert (b"memory" in lib.ci_last_error()) == refused, lib.ci_last_error()
+
+
+def test_more_work_than_a_list_counts_is_refused():
+    from comp_inference_amd import _lib
+
+    lib = _lib.lib()
+    a = _Args()
+    a.batch.num_tokens, a.batch.table_width, a.batch.table_stride = 1 << 24, 1 << 18, 1 << 18
+    a.q, a.out = _placed(0), _placed(1 << 40)
+    rc = a.attend(lib)
+    assert rc != 0 and (b"several" in lib.ci_last_error() or not torch.cuda.is_available()), lib.ci_last_error()
+
+
 def test_sizes_of_a_cache():
     from comp_inference_amd import attention_hip as A
 
