@@ -5,8 +5,9 @@
 //   (no window, or p - j < window, or j < sinks)
 //
 // One pass over the keys with a running maximum and sum per row (both, and the output, in 32 bits; weights are rounded to
-// bf16 for the matrix instruction, one rounding of 2^-9 each, while their sum takes them unrounded).  The query heads that
-// share a kv head are rows of one product: row r of a sequence's kv head is (token r / group, head r % group).
+// bf16 for the matrix instruction, off by at most 2^-8 of themselves each, while their sum takes them unrounded).  The
+// query heads that share a kv head are rows of one product: row r of a sequence's kv head is (token r / group, head
+// r % group).
 //
 // S^T = K Q^T puts queries into columns, so a lane holds 16 scores of ONE row and maximum and sum are lane arithmetic plus
 // one exchange between lane halves, and P^T is the operand of O^T = V^T P^T as it stands.
@@ -15,9 +16,15 @@
 //   attend_split_kernel   for few rows (single tokens): bound by reading the cache.  A tile is up to 32 rows; the blocks of
 //                         keys of all (sequence, tile, head) items form one list that is cut into equal shares, one per
 //                         workgroup, wherever the cut falls, so a batch of very different lengths fills the chip evenly.
-//                         An item that was cut is joined by attend_join_kernel.
-//   attend_rows_kernel    for many rows (prompts): bound by the matrix and vector units.  Four wavefronts of 32 rows share
-//                         the keys and values of a step of 64 tokens through the LDS.
+//                         An item that was cut is joined by attend_join_kernel.  Measured, 32 heads over 8 of 128 (a
+//                         copy on the same card moves 4.9 TB/s, read and written): one token each of 4 documents of 60
+//                         to 131 thousand tokens, 1.6 GB: 270 us, 5.8 TB/s; of 64 ragged chats under a window of 4096,
+//                         1.0 GB: 186 us, 5.4 TB/s; of 48 ragged chats in 4 bits, 0.86 GB: 184 us, 4.7 TB/s.
+//   attend_rows_kernel    for many rows (prompts): bound by the matrix and vector units.  Eight wavefronts of 32 rows share
+//                         the keys and values of a step of 64 tokens through the LDS, in two groups that take turns at the
+//                         matrix unit.  Measured, the same heads: a prompt of 8192 tokens 553 us, 0.99 PFLOP/s (a large
+//                         library product reaches 1.20); the last 1500 tokens each of two sequences of up to 16384 in
+//                         4 bits 930 us, 0.63 PFLOP/s, where the vector unit has the steps and middles to apply as well.
 #include "paged.h"
 
 namespace ci {
@@ -287,7 +294,7 @@ struct Cols {
 template <int D>
 struct Running {
     f32x16_p o[D / 32];
-    float m, l, off;  // off: what the 128 + code form of 4-bit values adds, to be taken out
+    float m, l, off;  // off: 4 bits: the part of the output that all channels share (sum of weight times the values' middles)
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) o[i] = splat16(0.0f);
@@ -418,7 +425,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
 
     // bf16: a block's keys are asked for a step ahead and its values at the head of its own step (8 KB or more are then always on
     // their way).  4 bits: a block is a quarter of that, so the next one is asked for whole, with its (step, low) pairs,
-    // before this one is begun (48 chats of up to 32 k tokens: 214 us as for bf16, 195 so; two blocks at a time 205).
+    // before this one is begun (48 chats of up to 32 k tokens: 214 us as for bf16, 195 so, 184 since codes become
+    // operands in two instructions a pair; two blocks at a time 205).
     constexpr bool kPairsAhead = NV <= 8;  // (registers do not go further)
     const CodeMask codes;
     Data x, y;
@@ -754,7 +762,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
 // ---- many rows ------------------------------------------------------------------------------------------------------
 constexpr uint32_t kStep = 64;  // keys
 constexpr uint32_t kRowWaves = 8, kRowThreads = 64 * kRowWaves, kTileRows = 32 * kRowWaves;
-constexpr uint32_t rows_lds(uint32_t kind, uint32_t D) {  // two buffers of two blocks, keys and values in bf16; steps and lows
+constexpr uint32_t rows_lds(uint32_t kind, uint32_t D) {  // two buffers of two blocks, keys and values in bf16; steps and mids
     return 2 * 2 * 128 * D + (kind == CI_KV_BF16 ? 0 : 4 * 256 * 4);
 }
 // Workgroups resident on a CU: registers allow two wavefronts per SIMD, four for heads of 64 in bf16.
@@ -770,8 +778,9 @@ struct Blocks {  // the two blocks of a step
 template <int KIND, int D>
 struct Stage;
 
-// The keys behind the end of a sequence need not be numbers; their scores are set, and their values are put to zero here.
-// `held` has a bit for every token of the block that is there (all ones: nothing to do).
+// The keys behind the end of a sequence need not be numbers; their scores are set, and their values (in 4 bits what these
+// are scaled by) are put to zero here: clear(keys0, keys1, held0, held1) has a bit for every token that is there of the two
+// blocks whose keys, and of the two whose values are staged.
 
 // bf16: blocks are copied as they lie.
 template <int D>
@@ -1096,9 +1105,9 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         phase_end();
         // ---- matrix phase (behind the last step: the scores of what lies there, for nothing)
         __builtin_amdgcn_s_setprio(1);
-        // (in the order that keeps the matrix unit fed: turning codes into values takes the vector unit a while, and runs
-        // beside the first half's matrix instructions; copies are best out of the way first.  The other way round: a 4-bit
-        // prompt part 892 instead of 816 us, a bf16 prompt 658 instead of 552)
+        // (in the order that keeps the matrix unit fed: turning codes into numbers takes the vector unit a while, and runs
+        // beside the first half's matrix instructions; copies are best out of the way first.  The other way round: the 4-bit
+        // prompt part 1100 instead of 925 us, the bf16 prompt of 8192 tokens 645 instead of 553)
         if (KIND != CI_KV_BF16) output(st);
         put(st + 2);
         ask(st + 3);
@@ -1313,7 +1322,7 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     if (p->many) {
         p->workers = p->grid = (cus * row_groups(kind, head_dim) + 7) / 8 * 8;
         // tiles of few steps: one workgroup each, handed out by the hardware, and nothing to join (ragged prompts of up to 6001
-        // tokens under a window of 1000: 153 us in shares, 124 whole)
+        // tokens under a window of 1000: 152 us in shares, 124 whole)
         uint64_t keys = longest;
         const uint64_t reach = (uint64_t)window + sinks + kTileRows / group + 3 * kStep;
         if (window && reach < keys) keys = reach;
@@ -1326,7 +1335,7 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     if (window && (uint64_t)window + sinks + 64 < keys) keys = (uint64_t)window + sinks + 64;
     p->whole = keys <= 4 * kUnit * kKvBlock;
     // as many as are resident; for 4 bits, where a workgroup waits longer for its first block than it then reads, twice as many
-    // if each still has much to do (48 chats of up to 32 k tokens 195 -> 187 us; one document of 65 k would lose, 28 -> 36)
+    // if each still has much to do (48 chats of up to 32 k tokens 203 -> 195 us; one document of 65 k would lose, 28 -> 37)
     const uint64_t units = (uint64_t)b.seqs * v.kv_heads * (keys / (kUnit * kKvBlock));
     p->workers = (kind != CI_KV_BF16 && units >= 64ull * cus ? 4 : 2) * cus;
     p->grid = p->whole ? p->items : p->workers;

@@ -78,7 +78,6 @@ CI_SIM_MINMAX(double)
 #define __builtin_amdgcn_s_barrier() sim::syncthreads()
 #define __builtin_amdgcn_sched_barrier(mask) ((void)0)
 #define __builtin_amdgcn_s_setprio(n) ((void)0)
-
 #define __shfl(v, src, width) sim::shfl((int)(v), (int)(src), (int)(width))
 #define __shfl_up(v, d, width) sim::shfl_up((int)(v), (unsigned)(d), (int)(width))
 
