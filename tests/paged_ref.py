@@ -86,12 +86,12 @@ def attention(q, k, v, first, scale, window=0, sinks=0):
     return out, lse.reshape(n, H), mass, worst
 
 
-def attention_bound(out, mass, worst, dim, values_rounded=False):
+def attention_bound(out, mass, worst, dim):
     """How far an element may be off.  Weights are rounded to bf16 once (half a step each: HALF_STEP of sum w |v|), the
-    output once (HALF_STEP of it); `values_rounded`: the values once more, on the way.  A score is a 32-bit sum of `dim`
+    output once (HALF_STEP of it).  A score is a 32-bit sum of `dim`
     products, each addition off by 2^-24 of a partial sum of at most `worst`, then scaled and exponentiated (2^-21 of the
     largest power): twice its error, relative, moves a weight and the sum of weights.  4-bit operands carry 128 + code, at
     most 16 times what a code stands for, through the same 32-bit sums."""
     score = dim * 16 * worst * 2.0 ** -24 + 2.0 ** -21 * (worst + 1.0)
-    weight = HALF_STEP * (2 if values_rounded else 1) + 2 * score + dim * 16 * 2.0 ** -24
+    weight = HALF_STEP + 2 * score + dim * 16 * 2.0 ** -24
     return 1.02 * weight * mass + 1.02 * HALF_STEP * out.abs() + 1e-30
