@@ -351,16 +351,14 @@ __device__ __forceinline__ uint32_t tiles_of(const AttendArgs &a, const SeqInfo 
 // Units of a sequence over all its tiles and heads.
 template <int RP>
 __device__ __forceinline__ uint32_t weight_of(const AttendArgs &a, uint32_t i) {
-    bool bad;
-    const SeqInfo s = load_seq(a.batch, a.cache, i, bad);
+    const SeqInfo s = load_seq_in_sum(a.batch, a.cache, i);
     uint32_t n = 0;
     for (uint32_t t = 0; t < tiles_of<RP>(a, s); ++t) n += units_of<RP>(a, s, t);
     return n * a.cache.kv_heads;
 }
 template <int RP>
 __device__ __forceinline__ uint32_t items_of(const AttendArgs &a, uint32_t i) {
-    bool bad;
-    return tiles_of<RP>(a, load_seq(a.batch, a.cache, i, bad)) * a.cache.kv_heads;
+    return tiles_of<RP>(a, load_seq_in_sum(a.batch, a.cache, i)) * a.cache.kv_heads;
 }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
@@ -1181,10 +1179,7 @@ __global__ __launch_bounds__(kRowThreads, 2 * row_groups(KIND, D)) void attend_r
     Found f;
     bool bad;
     if (a.whole) {  // one tile each, those with the most keys of a head first
-        const auto items = [&](uint32_t i) {
-            bool x;
-            return tiles_in(a, load_seq(a.batch, a.cache, i, x)).tiles * a.cache.kv_heads;
-        };
+        const auto items = [&](uint32_t i) { return tiles_in(a, load_seq_in_sum(a.batch, a.cache, i)).tiles * a.cache.kv_heads; };
         const auto mine = [&](uint32_t total) {
             const uint32_t run = (total + 7) / 8, k = blockIdx.x >> 3;
             return k < run ? (blockIdx.x & 7) * run + k : 0xFFFFFFFFu;
@@ -1197,10 +1192,7 @@ __global__ __launch_bounds__(kRowThreads, 2 * row_groups(KIND, D)) void attend_r
         return;
     }
     const uint32_t worker = (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
-    const auto weight = [&](uint32_t i) {
-        bool x;
-        return tiles_in(a, load_seq(a.batch, a.cache, i, x)).head * a.cache.kv_heads;
-    };
+    const auto weight = [&](uint32_t i) { return tiles_in(a, load_seq_in_sum(a.batch, a.cache, i)).head * a.cache.kv_heads; };
     if (!locate(a.batch.seqs, weight, [&](uint32_t total) { return worker * RowShare(total, gridDim.x).share; }, word, f)) return;
     const RowShare cuts(f.total, gridDim.x);
     uint32_t seq = f.seq, base = f.begin;  // of the list, where the sequence begins
@@ -1241,10 +1233,7 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
     __shared__ uint32_t word[10];
     const uint32_t k = blockIdx.x + 1;
     Found f;
-    const auto weight = [&](uint32_t i) {
-        bool x;
-        return tiles_in(a, load_seq(a.batch, a.cache, i, x)).head * a.cache.kv_heads;
-    };
+    const auto weight = [&](uint32_t i) { return tiles_in(a, load_seq_in_sum(a.batch, a.cache, i)).head * a.cache.kv_heads; };
     if (!locate(a.batch.seqs, weight, [&](uint32_t total) { return k * RowShare(total, workers).share; }, word, f)) return;
     const RowShare cuts(f.total, workers);
     bool bad;

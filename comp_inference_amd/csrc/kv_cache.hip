@@ -93,11 +93,7 @@ __device__ __forceinline__ Tile find_tile(const KvBatch &b, const KvView &v, uin
     bool bad = false;
     if (b.start) {
         Found f;
-        const auto tiles = [&](uint32_t i) {
-            bool x;
-            return tiles_of(load_seq(b, v, i, x));
-        };
-        if (!locate(b.seqs, tiles, [&](uint32_t) { return index; }, word, f)) return t;
+        if (!locate(b.seqs, [&](uint32_t i) { return tiles_of(load_seq_in_sum(b, v, i)); }, [&](uint32_t) { return index; }, word, f)) return t;
         seq = f.seq;
         begin = f.begin;
     }

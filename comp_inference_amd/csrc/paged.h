@@ -106,6 +106,15 @@ __device__ __forceinline__ void report_bad_index(const KvBatch &b) {
     if (b.status) atomicOr(b.status, (uint32_t)CI_STATUS_BAD_INDEX);
 }
 
+// The same inside a sum over all sequences, which also meets those that have no work of their own to say it (offsets that
+// fall, lengths outside the table without a new token): the first workgroup's sum reports them.
+__device__ __forceinline__ SeqInfo load_seq_in_sum(const KvBatch &b, const KvView &v, uint32_t i) {
+    bool bad;
+    const SeqInfo s = load_seq(b, v, i, bad);
+    if (bad && blockIdx.x == 0 && blockIdx.y == 0) report_bad_index(b);
+    return s;
+}
+
 // Page that holds block `blk` of a sequence, or kNoPage if the table names none of the cache's.
 __device__ __forceinline__ uint32_t page_of(const KvBatch &b, const KvView &v, uint32_t seq, uint32_t blk) {
     const uint32_t page = (uint32_t)b.table[(uint64_t)seq * b.table_stride + (blk >> v.page_shift)];
