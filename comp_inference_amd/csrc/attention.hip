@@ -680,8 +680,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
         const uint32_t per = (a.batch.seqs + 255) / 256, first = min(threadIdx.x * per, a.batch.seqs);
         const uint32_t end = min(first + per, a.batch.seqs);
         uint32_t mine = 0;
-        for (uint32_t i = first; i < end; ++i) mine += weight_of<RP>(a, i);
+        for (uint32_t i = first; i < end; ++i) mine = add_work(mine, weight_of<RP>(a, i));
         before = scan_threads(mine, word, total);
+        if (total == kTooMuch) return;  // (the same in every thread)
         if (it.seq >= first && it.seq < end) {
             for (uint32_t i = first; i < it.seq; ++i) before += weight_of<RP>(a, i);
             word[8] = before;

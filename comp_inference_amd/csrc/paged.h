@@ -149,15 +149,21 @@ __device__ __forceinline__ uint8_t *block_at(const KvView &v, uint32_t page, uin
            (blk & ((1u << v.page_shift) - 1)) * KvBlock<KIND, D>::kBytes;  // (a page is below 4 GiB)
 }
 
-// Exclusive prefix sum over the threads of a workgroup (up to eight wavefronts); `total` gets the sum.  `part` holds eight
-// words of LDS.
+// Sums of work stop at the largest word.  The host has checked that the work of a batch stays below it, but for a batch
+// whose row offsets fall: rows then belong to several sequences, and the sum may be anything.  Wrapped around, it would
+// name places that do not exist; a sum that has reached kTooMuch is no sum, and nothing is done for that batch.
+constexpr uint32_t kTooMuch = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t add_work(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
+// Exclusive prefix sum over the threads of a workgroup (up to eight wavefronts); `total` gets the sum (kTooMuch: the prefixes
+// mean nothing).  `part` holds eight words of LDS.
 __device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t *part, uint32_t &total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t inc = x;
 #pragma unroll
     for (uint32_t d = 1; d < 64; d *= 2) {
         const uint32_t y = (uint32_t)__shfl_up((int)inc, d, 64);
-        if (lane >= d) inc += y;
+        if (lane >= d) inc = add_work(inc, y);
     }
     __syncthreads();
     if (lane == 63) part[wave] = inc;
@@ -166,8 +172,8 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t *part, uin
     total = 0;
     for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
         const uint32_t p = part[w];
-        if (w < wave) before += p;
-        total += p;
+        if (w < wave) before = add_work(before, p);
+        total = add_work(total, p);
     }
     return before + inc - x;
 }
@@ -183,9 +189,10 @@ template <typename W, typename T>
 __device__ __forceinline__ bool locate(uint32_t seqs, W weight, T target, uint32_t *word, Found &f) {
     const uint32_t per = (seqs + blockDim.x - 1) / blockDim.x, first = min(threadIdx.x * per, seqs), last = min(first + per, seqs);
     uint32_t mine = 0;
-    for (uint32_t i = first; i < last; ++i) mine += weight(i);
+    for (uint32_t i = first; i < last; ++i) mine = add_work(mine, weight(i));
     uint32_t at = scan_threads(mine, word, f.total);
     f.total = (uint32_t)__builtin_amdgcn_readfirstlane((int)f.total);
+    if (f.total == kTooMuch) return false;
     f.target = target(f.total);
     if (f.target >= f.total) return false;
     if (f.target >= at && f.target - at < mine) {
