@@ -59,6 +59,7 @@ __device__ __forceinline__ float other_half(float x) {  // the value of lane ^ 3
 __device__ __forceinline__ float lane_xor(float x, int d) {
     return __int_as_float(__shfl(__float_as_int(x), (int)(threadIdx.x & 63) ^ d, 64));
 }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 __device__ __forceinline__ float max_halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -91,6 +92,10 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, const SeqInfo &s, u
     }
     x.nb = x.s1 + end - x.w0;
     return x;
+}
+
+__device__ __forceinline__ int32_t position_of(const AttendArgs &a, const SeqInfo &s, uint32_t row) {
+    return s.len - s.n + (int32_t)token_of(a, row);
 }
 
 // Whether every row of the span sees every key of the block that starts at kb.
@@ -159,91 +164,6 @@ __device__ __forceinline__ Queries<D> load_queries(const AttendArgs &a, const Se
     q.sum += other_half(q.sum);
     return q;
 }
-
-// ---- one row, the plain way -----------------------------------------------------------------------------------------
-// A wavefront goes over the keys of one row, 64 at a time, and adds up only what the row sees.  In the kernels below a
-// matrix instruction multiplies the values of keys that SOME row of its tile sees by weights that are zero for the others;
-// where such a value is an infinity or a NaN, and where a page was none of the cache's (its keys are unseen), the row's
-// result comes out as no number, and the row is done again here.  Slow, and right.
-template <int KIND, int D>
-__device__ __forceinline__ void attend_one_row(const AttendArgs &a, uint32_t seq, const SeqInfo &s, uint32_t head, uint32_t row) {
-    const uint32_t lane = threadIdx.x & 63, tok = token_of(a, row), gh = head * a.group + row - tok * a.group;
-    const int32_t p = s.len - s.n + (int32_t)tok;
-    const uint16_t *q = a.q + (int64_t)(s.row + (int32_t)tok) * a.q_row + (int64_t)gh * a.q_head;
-    float m = kNone, l = 0.0f, o[D / 64];
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] = 0.0f;
-#pragma unroll 1
-    for (int32_t base = 0; base <= p; base += 64) {
-        const int32_t j = base + (int32_t)lane;
-        bool seen = j <= p && (!a.window || p - j < a.window || j < a.sinks);
-        if (!__builtin_amdgcn_ballot_w64(seen)) continue;
-        const uint32_t page = seen ? page_of(a.batch, a.cache, seq, (uint32_t)j / kKvBlock) : kNoPage;
-        seen = page != kNoPage;
-        const uint64_t who = __builtin_amdgcn_ballot_w64(seen);
-        if (!who) continue;
-        const uint8_t *block = block_at<KIND, D>(a.cache, seen ? page : 0, head, (uint32_t)j / kKvBlock);
-        const uint32_t t = (uint32_t)j % kKvBlock;
-        float x = 0.0f;
-        const uint32_t *pairs = reinterpret_cast<const uint32_t *>(block + KvBlock<KIND, D>::kPairs);
-        const uint32_t kp = KIND == CI_KV_BF16 ? 0 : pairs[t];
-#pragma unroll 1
-        for (uint32_t c = 0; c < D / 8; ++c) {
-            const u32x4 y = *reinterpret_cast<const u32x4 *>(q + 8 * c);
-            u32x4 k{};
-            uint32_t word = 0;
-            if (KIND == CI_KV_BF16)
-                k = reinterpret_cast<const u32x4 *>(block)[key_operand(c, t)];
-            else
-                word = reinterpret_cast<const uint32_t *>(block)[key_word(c, t)];
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                const float ye = e & 1 ? bf16_hi(y[e / 2]) : bf16_lo(y[e / 2]);
-                const float ke = KIND != CI_KV_BF16 ? fmaf((float)(word >> nibble_shift(e) & 15u), bf16_lo(kp), bf16_hi(kp))
-                                 : e & 1            ? bf16_hi(k[e / 2])
-                                                    : bf16_lo(k[e / 2]);
-                x = fmaf(ye, ke, x);
-            }
-        }
-        x = seen ? x * a.scale_log2 : kNone;
-        float top = most(m, x);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) top = most(top, lane_xor(top, d));
-        const float f = m == kNone ? 0.0f : exp2_fast(m - top);
-        float w = seen && top != kNone ? exp2_fast(x - top) : 0.0f, sum = w;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) sum += lane_xor(sum, d);
-        l = l * f + sum;
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) o[i] *= f;
-        m = top;
-#pragma unroll 1
-        for (uint32_t k = 0; k < 64; ++k) {
-            if (!(who >> k & 1)) continue;
-            const float wk = __int_as_float(__shfl(__float_as_int(w), (int)k, 64));
-            const uint32_t pk = (uint32_t)__shfl((int)page, (int)k, 64), blk = (uint32_t)(base + (int32_t)k) / kKvBlock, tk = (uint32_t)(base + (int32_t)k) % kKvBlock;
-            const uint8_t *vals = block_at<KIND, D>(a.cache, pk, head, blk) + KvBlock<KIND, D>::kHalf;
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) {
-                const uint32_t at = value_operand<D>(lane + 64 * i, tk), e = value_element(tk);
-                float v;
-                if (KIND == CI_KV_BF16) {
-                    v = bf16_lo(reinterpret_cast<const uint16_t *>(vals)[at * 8 + e]);
-                } else {
-                    const uint32_t vp = reinterpret_cast<const uint32_t *>(vals - KvBlock<KIND, D>::kHalf + KvBlock<KIND, D>::kPairs)[kKvBlock + tk];
-                    v = fmaf((float)(reinterpret_cast<const uint32_t *>(vals)[value_word(at)] >> nibble_shift(e) & 15u), bf16_lo(vp), bf16_hi(vp));
-                }
-                o[i] += wk * v;
-            }
-        }
-    }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) dst[lane + 64 * i] = (uint16_t)bf16_pair(o[i] * inv, 0.0f);
-    if (a.lse && lane == 0) a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
-}
-__device__ __forceinline__ bool no_number(float x) { return !(fabsf(x) < __builtin_inff()); }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
 // RP columns of the 32 are rows; the columns c, c + RP, c + 2 RP .. hold the same row.  Every one of them gets all 32 scores
@@ -316,6 +236,15 @@ struct Running {
         }
     }
     __device__ __forceinline__ float base() const { return m == kNone ? 0.0f : m; }
+    // whether something that was summed is an infinity or a NaN
+    __device__ __forceinline__ bool no_number() const {
+        float x = l * 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x = fmaf(o[i][k], 0.0f, x);
+        return x != x;
+    }
 };
 
 // A value operand (s, h) without the keys that no row sees (what lies there need not be a number); `seen` has the lane's
@@ -334,6 +263,169 @@ struct BlockData {  // keys and values of one block, as they lie in the cache
     static constexpr int N = KIND == CI_KV_BF16 ? D / 16 : D / 64;
     u32x4 k[N], v[N];
 };
+
+// Scores of a lane's keys of one block, from q . k (4 bits: q . (128 + code)); keys the row does not see get kNone.  `sees`:
+// the lane's keys that its row sees, the share's first key as bit 0, looked at where `edge`.
+template <int KIND, int D, int RP>
+__device__ __forceinline__ void weigh_block(const AttendArgs &a, const Cols<RP> &cols, float q_sum, Running<D> &run, const f32x16_p &acc,
+                                            bool edge, uint32_t sees, const uint32_t (&kp)[Cols<RP>::NV],
+                                            const uint32_t (&vp)[Cols<RP>::NV], uint32_t (&pk)[Cols<RP>::NV / 2]) {
+    constexpr int NV = Cols<RP>::NV;
+    float t[NV];
+    cols.take(acc, t);
+    float best = kNone;
+#pragma unroll
+    for (int e = 0; e < NV; ++e) {
+        // (q . (low + step code) from q . (128 + code))
+        if (KIND != CI_KV_BF16) t[e] = (t[e] - 128.0f * q_sum) * bf16_lo(kp[e]) + q_sum * bf16_hi(kp[e]);
+        t[e] *= a.scale_log2;
+        if (edge) t[e] = sees >> ((e & 3) + 8 * (e >> 2)) & 1 ? t[e] : kNone;
+        best = most(best, t[e]);
+    }
+    run.raise(max_halves(best));
+    const float base = run.base();
+#pragma unroll
+    for (int e = 0; e < NV; e += 2) {
+        const float p0 = exp2_fast(t[e] - base), p1 = exp2_fast(t[e + 1] - base);
+        run.l += p0 + p1;
+        if (KIND == CI_KV_BF16) {
+            pk[e / 2] = bf16_pair(p0, p1);
+        } else {
+            // o = sum p (low + step code): the step goes into the weight r = p step, which is rounded, and what is added back
+            // in 32 bits is sum p (low + 7.5 step) - sum r 135.5, so that the rounding of r meets code - 7.5 (as large as
+            // the value is away from its row's middle) and not the code, or 128 with it.  A key that is not seen weighs
+            // nothing, whatever its step and low are
+            const float s0 = p0 * bf16_lo(vp[e]), s1 = p1 * bf16_lo(vp[e + 1]);
+            float l0 = fmaf(s0, 7.5f, p0 * bf16_hi(vp[e])), l1 = fmaf(s1, 7.5f, p1 * bf16_hi(vp[e + 1]));
+            pk[e / 2] = bf16_pair(s0, s1);
+            if (edge) {
+                const bool z0 = t[e] == kNone, z1 = t[e + 1] == kNone;
+                l0 = z0 ? 0.0f : l0;
+                l1 = z1 ? 0.0f : l1;
+                pk[e / 2] &= (z0 ? 0u : 0xFFFFu) | (z1 ? 0u : 0xFFFF0000u);
+            }
+            run.off += l0 + l1 - 135.5f * (bf16_lo(pk[e / 2]) + bf16_hi(pk[e / 2]));
+        }
+    }
+}
+
+// ---- blocks done again ----------------------------------------------------------------------------------------------
+// A matrix instruction multiplies the values of keys that SOME column of a tile takes by weights that are zero for the others;
+// where such a value is an infinity or a NaN, and where a page was none of the cache's, sums come out as no numbers that
+// should not.  A wavefront that finds one does its blocks again, with attend_again.
+//
+// Such values are taken out of the operands there, and what they are to the rows that do see them is found by a second
+// product, of ones for the keys a column takes and of 1 for +infinity, 64 for -infinity, 4096 for NaN: up to 32 keys of each
+// kind, counted exactly.
+//
+// Measured with a NaN in a channel of the first value, which every row sees: a prompt of 8192 tokens, 32 heads over 8 of 128,
+// 3.3 ms instead of 0.6; one token each over 20000, 45 us instead of 28.
+constexpr uint32_t kBf16One = 0x3F80u;
+
+// A value operand without them; `most` is raised to the largest exponent (in place).
+__device__ __forceinline__ u32x4 without_wild(u32x4 v, uint32_t &most) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t lo = v[w] & 0x7F80u, hi = v[w] >> 16 & 0x7F80u;
+        most = max(most, max(lo, hi));
+        if (lo == 0x7F80u) v[w] &= 0xFFFF0000u;
+        if (hi == 0x7F80u) v[w] &= 0xFFFFu;
+    }
+    return v;
+}
+// What they are, as numbers to count by.
+__device__ __forceinline__ u32x4 kinds_of_wild(u32x4 v) {
+    const auto kind = [](uint32_t x) { return x == 0x7F80u ? kBf16One : x == 0xFF80u ? 0x4280u : (x & 0x7F80u) == 0x7F80u ? 0x4580u : 0u; };
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[w] = kind(v[w] & 0xFFFFu) | kind(v[w] >> 16) << 16;
+    return v;
+}
+
+// Sums of one wavefront's blocks block(i0), block(i0 + step) .. before `end` anew, for rows r0 .. r1 - 1.  Pages that do not
+// exist are left out.  Nothing is asked for ahead and nothing is held from block to block but the sums (with heads of 64 a
+// wavefront has 128 registers).
+template <int KIND, int D, int RP, typename B>
+__device__ __forceinline__ void attend_again(const AttendArgs &a, uint32_t seq, const SeqInfo &s, uint32_t head, uint32_t r0, uint32_t r1,
+                                             uint32_t i0, uint32_t end, uint32_t step, B block, Running<D> &run) {
+    constexpr int N = BlockData<KIND, D>::N, NV = Cols<RP>::NV;
+    const uint32_t lane = threadIdx.x & 63, h = lane >> 5;
+    const Cols<RP> cols;
+    const CodeMask codes;
+    run.clear();
+#pragma unroll 1
+    for (uint32_t i = i0; i < end; i += step) {
+        const uint32_t blk = block(i);
+        const int32_t kb = (int32_t)(blk * kKvBlock);
+        if (kb >= s.len) continue;
+        const uint32_t page = uniform(page_of(a.batch, a.cache, seq, blk));
+        if (page == kNoPage) continue;
+        const uint8_t *b = block_at<KIND, D>(a.cache, page, head, blk);
+        asm volatile("" : "+s"(r0) : : "memory");  // (what is derived from it, or was asked for before, is so again)
+        const uint32_t row = r0 + (lane & 31) % RP;
+        const int32_t pos = position_of(a, s, row), p_lo = position_of(a, s, r0), p_hi = position_of(a, s, r1 - 1);
+        const uint32_t sees = seen_keys(a, pos, pos, kb) >> cols.key0;
+        f32x16_p acc = splat16(0.0f);
+        uint32_t kp[NV], vp[NV], pk[NV / 2];
+        float sum;
+        {
+            const Queries<D> q = load_queries<D>(a, s, head, row, r1);
+            u32x4 x[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) x[k] = reinterpret_cast<const u32x4 *>(b)[k * 64 + lane];
+            if (KIND != CI_KV_BF16) {
+                const uint32_t *pairs = reinterpret_cast<const uint32_t *>(b + KvBlock<KIND, D>::kPairs);
+                cols.pairs(pairs, kp);
+                cols.pairs(pairs + kKvBlock, vp);
+            }
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                acc = mfma(KIND == CI_KV_BF16 ? x[k % N] : codes.to_bf16(x[k / 4 % N][k % 4]), q.f[k], acc);
+            sum = q.sum;
+        }
+        weigh_block<KIND, D, RP>(a, cols, sum, run, acc, true, sees, kp, vp, pk);
+        const uint32_t seen = seen_keys(a, p_lo, p_hi, kb) >> (4 * h);
+        const auto value = [&](int s2, int db) {
+            const int o = s2 * (D / 32) + db;
+            const uint8_t *v = b + KvBlock<KIND, D>::kHalf;
+            if (KIND != CI_KV_BF16) return codes.to_bf16(reinterpret_cast<const uint32_t *>(v)[(o / 4 * 64 + lane) * 4 + o % 4]);
+            return keep_seen(reinterpret_cast<const u32x4 *>(v)[o * 64 + lane], seen, (uint32_t)s2);
+        };
+        uint32_t wild = 0;
+        {
+            u32x4 f[2];
+            cols.give(pk, f);
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db) {
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
+                    run.o[db] = mfma(KIND == CI_KV_BF16 ? without_wild(value(s2, db), wild) : value(s2, db), f[s2], run.o[db]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (KIND != CI_KV_BF16 || !__builtin_amdgcn_ballot_w64(wild == 0x7F80u)) continue;
+#pragma unroll
+        for (int e = 0; e < NV; e += 2) {
+            const uint32_t two = sees >> ((e & 3) + 8 * (e >> 2));
+            pk[e / 2] = ((two & 1) ? kBf16One : 0u) | ((two & 2) ? kBf16One << 16 : 0u);
+        }
+        u32x4 ones[2];
+        cols.give(pk, ones);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+            asm volatile("" ::: "memory");
+            f32x16_p kinds = mfma(kinds_of_wild(value(0, db)), ones[0], splat16(0.0f));
+            kinds = mfma(kinds_of_wild(value(1, db)), ones[1], kinds);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const uint32_t n = (uint32_t)kinds[k];
+                if (n & 63) run.o[db][k] += __builtin_inff();
+                if (n >> 6 & 63) run.o[db][k] -= __builtin_inff();
+                if (n >> 12) run.o[db][k] = __builtin_nanf("");
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (32 channels after the other: registers)
+        }
+    }
+}
 
 struct Item {
     uint32_t seq, tile, head;
@@ -360,8 +452,6 @@ template <int RP>
 __device__ __forceinline__ uint32_t items_of(const AttendArgs &a, uint32_t i) {
     return tiles_of<RP>(a, load_seq_in_sum(a.batch, a.cache, i)) * a.cache.kv_heads;
 }
-
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
 // Item number `index` of the batch.
 template <int RP>
@@ -412,7 +502,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
         for (int i = 0; i < Data::N; ++i) x.v[i] = reinterpret_cast<const u32x4 *>(b + KvBlock<KIND, D>::kHalf)[i * 64 + lane];
     };
     PageRun table(a.batch, it.seq);
-    // the block of a step (of a page that is none of the cache's: page 0; the item's rows are done again)
+    // the block of a step (of a page that is none of the cache's: page 0; the blocks are done again)
     auto place = [&](uint32_t i) -> const uint8_t * {
         const uint32_t blk = span.block(i);
         table.hold(a.batch, a.cache, blk);
@@ -466,43 +556,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             b = place(min(i + kUnit, last - 1));
             fetch_k(b, x);
         }
-        float t[NV];
-        cols.take(acc, t);
-        float best = kNone;
-#pragma unroll
-        for (int e = 0; e < NV; ++e) {
-            // (q . (low + step code) from q . (128 + code))
-            if (KIND != CI_KV_BF16) t[e] = (t[e] - 128.0f * q.sum) * bf16_lo(kp[e]) + q.sum * bf16_hi(kp[e]);
-            t[e] *= a.scale_log2;
-            if (edge) t[e] = sees >> ((e & 3) + 8 * (e >> 2)) & 1 ? t[e] : kNone;
-            best = most(best, t[e]);
-        }
-        run.raise(max_halves(best));
-        const float base = run.base();
         uint32_t pk[NV / 2];
-#pragma unroll
-        for (int e = 0; e < NV; e += 2) {
-            const float p0 = exp2_fast(t[e] - base), p1 = exp2_fast(t[e + 1] - base);
-            run.l += p0 + p1;
-            if (KIND == CI_KV_BF16) {
-                pk[e / 2] = bf16_pair(p0, p1);
-            } else {
-                // o = sum p (low + step code): the step goes into the weight r = p step, which is rounded, and what is added back
-                // in 32 bits is sum p (low + 7.5 step) - sum r 135.5, so that the rounding of r meets code - 7.5 (as large as
-                // the value is away from its row's middle) and not the code, or 128 with it.  A key that is not seen weighs
-                // nothing, whatever its step and low are
-                const float s0 = p0 * bf16_lo(vp[e]), s1 = p1 * bf16_lo(vp[e + 1]);
-                float l0 = fmaf(s0, 7.5f, p0 * bf16_hi(vp[e])), l1 = fmaf(s1, 7.5f, p1 * bf16_hi(vp[e + 1]));
-                pk[e / 2] = bf16_pair(s0, s1);
-                if (edge) {
-                    const bool z0 = t[e] == kNone, z1 = t[e + 1] == kNone;
-                    l0 = z0 ? 0.0f : l0;
-                    l1 = z1 ? 0.0f : l1;
-                    pk[e / 2] &= (z0 ? 0u : 0xFFFFu) | (z1 ? 0u : 0xFFFF0000u);
-                }
-                run.off += l0 + l1 - 135.5f * (bf16_lo(pk[e / 2]) + bf16_hi(pk[e / 2]));
-            }
-        }
+        weigh_block<KIND, D, RP>(a, cols, q.sum, run, acc, edge, sees, kp, vp, pk);
         u32x4 f[2];
         cols.give(pk, f);
         if (KIND == CI_KV_BF16 && edge) {
@@ -525,15 +580,14 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             }
         }
     }
-    if (lost) {
-        if (lane == 0) report_bad_index(a.batch);
-        run.l = __builtin_nanf("");  // (the rows will be found to be no numbers, and done again)
-    }
+    if (lost && lane == 0) report_bad_index(a.batch);
+    if (__builtin_amdgcn_ballot_w64(row < rows && (lost || run.no_number())))
+        attend_again<KIND, D, RP>(a, it.seq, s, it.head, r0, r0 + rows, u0 * kUnit + wave, last, kUnit,
+                                  [&](uint32_t k) { return span.block(k); }, run);
 
     // ---- join: the columns of a wavefront that hold the same row (c, c + RP, ..), then the four wavefronts
     float *o_lds = reinterpret_cast<float *>(lds);                      // [4][32][kStride]
     float *m_lds = o_lds + 4 * 32 * kStride, *l_lds = m_lds + 4 * RP;  // [4][RP] each
-    uint32_t *again = reinterpret_cast<uint32_t *>(l_lds + 4 * RP);    // rows that are no numbers, a bit each
     run.l += other_half(run.l);
     run.off += other_half(run.off);
     float m = run.m;
@@ -544,7 +598,6 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
 #pragma unroll
     for (int d = RP; d < 32; d *= 2) l += lane_xor(l, d);
     __syncthreads();  // (the LDS is free of the piece before)
-    if (threadIdx.x == 0) *again = 0;
     if (lane < RP) {
         m_lds[wave * RP + lane] = m;
         l_lds[wave * RP + lane] = l;
@@ -579,7 +632,6 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing: zeros)
             const uint32_t tok = token_of(a, r0 + rr), g = r0 + rr - tok * a.group;
             u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
-            if (no_number(acc[0] * inv + acc[1] * inv + (acc[2] * inv + acc[3] * inv))) atomicOr(again, 1u << rr);
             *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row +
                                        (int64_t)(it.head * a.group + g) * a.o_head + d) = w;
             if (a.lse && d == 0)
@@ -593,16 +645,11 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             }
         }
     }
-    if (whole) {
-        __syncthreads();
-        for (uint32_t rr = wave; rr < rows; rr += 4)
-            if (uniform(*again) >> rr & 1) attend_one_row<KIND, D>(a, it.seq, s, it.head, r0 + rr);
-    }
 }
 
 template <int D, int RP>
 constexpr uint32_t slot_floats() { return RP * (D + 2); }
-constexpr uint32_t split_lds(int D) { return (4 * 32 * (D + 4) + 2 * 4 * 32 + 4) * 4; }
+constexpr uint32_t split_lds(int D) { return (4 * 32 * (D + 4) + 2 * 4 * 32) * 4; }
 
 // Units of all items in the order (sequence, tile, head), cut evenly.
 __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t workers) { return max((total + workers - 1) / workers, 1u); }
@@ -730,7 +777,6 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
     }
     *reinterpret_cast<f32x4_p *>(part + threadIdx.x * 4) = acc;
     if (d == 0) part_l[g] = l, part_m[g] = m;
-    if (threadIdx.x == 0) word[0] = 0;
     __syncthreads();
     if (threadIdx.x < kLanes) {
         m = kNone;
@@ -752,10 +798,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
         *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
         if (a.lse && d == 0)
             a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
-        if (no_number(acc[0] * inv + acc[1] * inv + (acc[2] * inv + acc[3] * inv))) atomicOr(word, 1u);
     }
-    __syncthreads();
-    if (threadIdx.x < 64 && uniform(word[0])) attend_one_row<KIND, D>(a, it.seq, s, it.head, r0 + row);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------
@@ -887,9 +930,6 @@ __device__ __forceinline__ Steps steps_between(const AttendArgs &a, int32_t p_lo
     }
     x.n = x.s1 + end - x.w0;
     return x;
-}
-__device__ __forceinline__ int32_t position_of(const AttendArgs &a, const SeqInfo &s, uint32_t row) {
-    return s.len - s.n + (int32_t)token_of(a, row);
 }
 __device__ __forceinline__ uint32_t steps_of(const AttendArgs &a, const SeqInfo &s, uint32_t tile) {
     const uint32_t r0 = tile * kTileRows, r1 = min(r0 + kTileRows, rows_of(a, s));
@@ -1116,12 +1156,12 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         phase_end();
     }
     if (u0 < last && !second) phase_end();  // (the second group's last phase)
-    if (lost) {
-        if (threadIdx.x == 0) report_bad_index(a.batch);
-        run.l = __builtin_nanf("");  // (the rows will be found to be no numbers, and done again)
-    }
-    const float l = run.l + other_half(run.l);
+    if (lost && threadIdx.x == 0) report_bad_index(a.batch);
     const bool mine = r0 + col < t1;
+    if (__builtin_amdgcn_ballot_w64(mine && (lost || run.no_number())))
+        attend_again<KIND, D, 32>(a, seq, s, head, r0, r1, 2 * u0, 2 * last, 1,
+                                  [&](uint32_t k) { return first_block(k / 2) + k % 2; }, run);
+    const float l = run.l + other_half(run.l);
     if (KIND != CI_KV_BF16) {
         const float off = run.off + other_half(run.off);
 #pragma unroll
@@ -1146,7 +1186,6 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         return;
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    float check = 0.0f;
     if (mine) {
         const uint32_t tok = token_of(a, r0 + col), gh = head * a.group + r0 + col - tok * a.group;
         uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
@@ -1156,19 +1195,13 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
             for (int k = 0; k < 4; ++k) {
                 float y[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    y[c] = run.o[db][4 * k + c] * inv;
-                    check = fmaf(y[c], 0.0f, check);  // (a NaN once one of them is no number)
-                }
+                for (int c = 0; c < 4; ++c) y[c] = run.o[db][4 * k + c] * inv;
                 u32x2 w = {bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3])};
                 *reinterpret_cast<u32x2 *>(dst + 32 * db + 8 * k + 4 * h) = w;
             }
         if (a.lse && h == 0)
             a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = run.m == kNone ? kNone : (run.m + log2f(l)) * 0.6931471805599453f;
     }
-    const uint64_t again = __builtin_amdgcn_ballot_w64(check != check);
-    for (uint32_t rows = (uint32_t)again | (uint32_t)(again >> 32); rows; rows &= rows - 1)
-        attend_one_row<KIND, D>(a, seq, s, head, r0 + (uint32_t)__builtin_ctz(rows));
 }
 
 template <int KIND, int D>
@@ -1252,8 +1285,6 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
     uint32_t w1 = (at + t.places - 1) / cuts.share;
     if (w1 > k && cuts.cut(w1 * cuts.share - at, t.places) == t.places) --w1;
     constexpr uint32_t kLanes = D / 4;
-    if (threadIdx.x == 0) word[0] = 0;  // rows that are no numbers, a bit each
-    __syncthreads();
     const uint32_t d = threadIdx.x % kLanes * 4;
     for (uint32_t r = r0 + threadIdx.x / kLanes; r < r1; r += 256 / kLanes) {
         float m = kNone, l = 0.0f;
@@ -1274,12 +1305,7 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
         *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
         if (a.lse && d == 0)
             a.lse[(int64_t)(s.row + (int32_t)tok) * a.l_row + gh] = m == kNone ? kNone : (m + log2f(l)) * 0.6931471805599453f;
-        if (no_number(acc[0] * inv + acc[1] * inv + (acc[2] * inv + acc[3] * inv))) atomicOr(word, 1u << (r - r0));
     }
-    __syncthreads();
-    const uint32_t again = uniform(word[0]);
-    for (uint32_t r = r0 + uniform(threadIdx.x >> 6); r < r1; r += 4)
-        if (again >> (r - r0) & 1) attend_one_row<KIND, D>(a, f.seq, s, head, r);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
