@@ -115,6 +115,16 @@ __device__ __forceinline__ uint32_t seen_keys(const AttendArgs &a, int32_t p_lo,
 }
 
 
+// One over a row's sum of weights.  The largest weight is at least one, so a sum of zero is that of a row that sees no key,
+// which gets zeros, or of one whose scores are all minus infinity, which is no number.
+__device__ __forceinline__ float inverse_sum(const AttendArgs &a, uint32_t seq, const SeqInfo &s, uint32_t row, float l) {
+    if (l > 0.0f || l != l) return 1.0f / l;
+    const Span x = span_of(a, s, row, row + 1);
+    for (uint32_t i = x.nb; i > 0; --i)  // (its own key's page is the last)
+        if (page_of(a.batch, a.cache, seq, x.block(i - 1)) != kNoPage) return __builtin_nanf("");
+    return 0.0f;
+}
+
 // ---- matrix operands ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ f32x16_p mfma(u32x4 x, u32x4 y, f32x16_p c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_p, x), __builtin_bit_cast(bf16x8_p, y), c, 0, 0, 0);
@@ -629,7 +639,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &a, const Item &it
             }
         }
         if (whole) {
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees nothing: zeros)
+            const float inv = inverse_sum(a, it.seq, s, r0 + rr, l);
             const uint32_t tok = token_of(a, r0 + rr), g = r0 + rr - tok * a.group;
             u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
             *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row +
@@ -792,7 +802,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] += f * y[c];
         }
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const float inv = inverse_sum(a, it.seq, s, r0 + row, l);
         const uint32_t tok = token_of(a, r0 + row), gh = it.head * a.group + r0 + row - tok * a.group;
         u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
         *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;
@@ -1185,8 +1195,8 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
         }
         return;
     }
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     if (mine) {
+        const float inv = inverse_sum(a, seq, s, r0 + col, l);
         const uint32_t tok = token_of(a, r0 + col), gh = head * a.group + r0 + col - tok * a.group;
         uint16_t *dst = a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head;
 #pragma unroll
@@ -1299,7 +1309,7 @@ __global__ __launch_bounds__(256) void attend_rows_join_kernel(AttendArgs a, uin
             for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f0 + y[c] * f1;
             m = top;
         }
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const float inv = inverse_sum(a, f.seq, s, r, l);
         const uint32_t tok = token_of(a, r), gh = head * a.group + r - tok * a.group;
         u32x2 w = {bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv)};
         *reinterpret_cast<u32x2 *>(a.out + (int64_t)(s.row + (int32_t)tok) * a.o_row + (int64_t)gh * a.o_head + d) = w;

@@ -597,7 +597,8 @@ uint32_t ci_debug_wait_limit(uint32_t looks);
  *   ci_paged_kv_read     the stored keys and values of the last tokens of every sequence as rows
  *   ci_paged_attention   out = softmax over the visible keys of scale * q k^T, times v: key j is visible to the query at
  *                        position p when j <= p and (window == 0, or p - j < window, or j < sinks).  Query head h reads
- *                        kv head h / (q_heads / kv_heads).  A row that sees no key gets zeros.  d_lse (or NULL): fp32
+ *                        kv head h / (q_heads / kv_heads).  A row that sees no key gets zeros, one
+ *                        whose scores are all -inf is NaN.  d_lse (or NULL): fp32
  *                        [rows, q_heads], row stride lse_stride: natural logarithm of the sum of exp(scores), -inf for
  *                        a row without keys.  With a window, pages that hold no key a new token sees need not be named
  *                        (any entry will do).  out shares no memory with q.  max_query_len / max_seq_len: the caller's bounds on the lengths (0: not
