@@ -94,6 +94,13 @@ def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, device
     return torch.cat((angle.cos(), angle.sin()), dim=1).to(torch.float32).to(device)
 
 
+def _no_gradient(*operands):
+    """There is no backward pass: a result without one would cut the graph silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        raise RuntimeError("the paged cache and attention are for inference: an operand requires a gradient "
+                           "(call under torch.no_grad(), or detach it)")
+
+
 def _elsewhere(name: str, t, cache: PagedKVCache):
     return RuntimeError(f"{name} is on {t.device}, the cache on {cache.data.device}")
 
@@ -168,8 +175,9 @@ def paged_kv_append(cache: PagedKVCache, k, v, block_table, seq_lens, query_star
     angle first; the rotation is exact up to its one rounding to bf16.  `q` [T, heads, head_dim] is turned the same way
     into `q_out` (`q` itself, or memory of its own; made if not given), which is returned.  Rows behind the last sequence, and
     sequences of length 0, are left as they were.  Tokens, pages and table rows that do not exist are left out and
-    reported by `device_status`."""
+    reported by `device_status`.  No gradients: operands that require one are refused."""
     _lib.require_device(cache.data)
+    _no_gradient(k, v, q)
     index, H = cache.data.get_device(), cache.kv_heads
     kr = _rows("k", k, cache, index, H, None)
     tokens = k.shape[0]
@@ -230,8 +238,9 @@ def paged_attention(q, cache: PagedKVCache, block_table, seq_lens, query_start=N
     will do).  `out` shares no memory with q.  `scale`: 1 / sqrt(head_dim) if not given; positive.  `max_query_len`, `max_seq_len`: what the caller
     knows about the longest sequence (0: nothing); they choose kernels, the results do not rest on them.  `return_lse`:
     also fp32 [T, heads], the natural logarithm of the sum of exp(scores).  Scores, sums and the output are held in 32
-    bits; the weights are rounded to bf16 for the product with v.  Inference only."""
+    bits; the weights are rounded to bf16 for the product with v.  No gradients: a q that requires one is refused."""
     _lib.require_device(cache.data)
+    _no_gradient(q)
     dev = cache.data.device
     index = cache.data.get_device()
     qr = _rows("q", q, cache, index, None, None)
