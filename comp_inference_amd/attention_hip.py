@@ -172,7 +172,7 @@ def paged_kv_append(cache: PagedKVCache, k, v, block_table, seq_lens, query_star
     """Stores the keys and values [T, kv_heads, head_dim] (bf16, any row and head strides that are multiples of 8) of a
     batch's new tokens: the last ones of every sequence.  With `rotary` (a table as `rotary_table` makes; channels d and
     d + rotary_dim / 2 form a pair, the channels behind rotary_dim stay) keys and queries are turned by their position's
-    angle first; the rotation is exact up to its one rounding to bf16.  `q` [T, heads, head_dim] is turned the same way
+    angle first, in 64 bits, rounded to 32 bits and then to bf16.  `q` [T, heads, head_dim] is turned the same way
     into `q_out` (`q` itself, or memory of its own; made if not given), which is returned.  Rows behind the last sequence, and
     sequences of length 0, are left as they were.  Tokens, pages and table rows that do not exist are left out and
     reported by `device_status`.  No gradients: operands that require one are refused."""

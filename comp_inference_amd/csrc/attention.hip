@@ -19,7 +19,7 @@
 //                         An item that was cut is joined by attend_join_kernel.  Measured, 32 heads over 8 of 128 (a
 //                         copy on the same card moves 4.9 TB/s, read and written): one token each of 4 documents of 60
 //                         to 131 thousand tokens, 1.6 GB: 270 us, 5.8 TB/s; of 64 ragged chats under a window of 4096,
-//                         1.0 GB: 186 us, 5.4 TB/s; of 48 ragged chats in 4 bits, 0.86 GB: 184 us, 4.7 TB/s.
+//                         1.0 GB: 187 us, 5.4 TB/s; of 48 ragged chats in 4 bits, 0.86 GB: 181 us, 4.7 TB/s.
 //   attend_rows_kernel    for many rows (prompts): bound by the matrix and vector units.  Eight wavefronts of 32 rows share
 //                         the keys and values of a step of 64 tokens through the LDS, in two groups that take turns at the
 //                         matrix unit.  Measured, the same heads: a prompt of 8192 tokens 553 us, 0.99 PFLOP/s (a large
@@ -1168,9 +1168,14 @@ __device__ __forceinline__ void attend_rows_piece(const AttendArgs &a, uint32_t 
     if (u0 < last && !second) phase_end();  // (the second group's last phase)
     if (lost && threadIdx.x == 0) report_bad_index(a.batch);
     const bool mine = r0 + col < t1;
-    if (__builtin_amdgcn_ballot_w64(mine && (lost || run.no_number())))
-        attend_again<KIND, D, 32>(a, seq, s, head, r0, r1, 2 * u0, 2 * last, 1,
-                                  [&](uint32_t k) { return first_block(k / 2) + k % 2; }, run);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(mine && (lost || run.no_number())) != 0, 0)) {
+        // (with steps and sums of its own: taking those above the loop is scheduled worse, 4-bit prompt part 943 instead of 924 us)
+        const Steps again = steps_between(a, position_of(a, s, t0), position_of(a, s, t1 - 1));
+        Running<D> anew;
+        attend_again<KIND, D, 32>(a, seq, s, head, r0, r1, 2 * u0, 2 * min(u1, again.n), 1,
+                                  [&](uint32_t k) { return (uint32_t)again.first_key(k / 2) / kKvBlock + k % 2; }, anew);
+        run = anew;
+    }
     const float l = run.l + other_half(run.l);
     if (KIND != CI_KV_BF16) {
         const float off = run.off + other_half(run.off);
@@ -1333,6 +1338,9 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     if (int rc = cu_count(&cus)) return rc;
     const uint64_t rows = (uint64_t)b.tokens * group;
     const uint64_t per_seq = (uint64_t)(b.start ? new_longest : 1) * group;
+    // Measured with few | many rows' kernel, 32 heads over 8 of 128 in bf16: 512 tokens from the first on 29 | 28 us, 1024 557 |
+    // 41; 64 tokens behind 8192 41 | 67; 16 times 16 tokens behind 8192 147 | 151.  In 4 bits: 512 tokens 21 | 39, 1024 563 | 63.
+    // The rule does not look at the keys: 256 tokens behind 32768 go to the kernel for few (392 | 168).
     p->many = per_seq >= 64 && rows * v.kv_heads / kTileRows >= cus / 4;
     p->whole = false;
     p->work_bytes = 0;
@@ -1348,7 +1356,8 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     if (p->many) {
         p->workers = p->grid = (cus * row_groups(kind, head_dim) + 7) / 8 * 8;
         // tiles of few steps: one workgroup each, handed out by the hardware, and nothing to join (ragged prompts of up to 6001
-        // tokens under a window of 1000: 152 us in shares, 124 whole)
+        // tokens under a window of 1000: 152 us in shares, 124 whole; 2 prompts of 2048, 12 heads of 64, 80 and 47, of 4096 110
+        // and 131)
         uint64_t keys = longest;
         const uint64_t reach = (uint64_t)window + sinks + kTileRows / group + 3 * kStep;
         if (window && reach < keys) keys = reach;
@@ -1359,9 +1368,13 @@ static int plan_attend(const KvView &v, const KvBatch &b, uint32_t kind, uint32_
     }
     uint64_t keys = longest;
     if (window && (uint64_t)window + sinks + 64 < keys) keys = (uint64_t)window + sinks + 64;
+    // (64 tokens over 512 each: 35 us in shares, 28 whole; over 2048 each 113 and 107, but there a batch of unlike lengths would
+    // wait for its longest)
     p->whole = keys <= 4 * kUnit * kKvBlock;
-    // as many as are resident; for 4 bits, where a workgroup waits longer for its first block than it then reads, twice as many
-    // if each still has much to do (48 chats of up to 32 k tokens 203 -> 195 us; one document of 65 k would lose, 28 -> 37)
+    // as many as are resident (48 ragged chats of up to 32768 tokens in bf16, one to four workgroups per CU: 620, 615, 654, 618
+    // us; with heads of 64 329, 283, 278, 306); for 4 bits, where a workgroup waits longer for its first block than it then
+    // reads, twice as many if each still has much to do (the same chats 261, 215, 223, 213, with heads of 64 184, 134, 119, 115;
+    // 16 over 16384 each, at the border, 68, 56, 77, 64; one document of 65531 would lose, 28 -> 36)
     const uint64_t units = (uint64_t)b.seqs * v.kv_heads * (keys / (kUnit * kKvBlock));
     p->workers = (kind != CI_KV_BF16 && units >= 64ull * cus ? 4 : 2) * cus;
     p->grid = p->whole ? p->items : p->workers;

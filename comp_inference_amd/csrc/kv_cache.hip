@@ -8,9 +8,11 @@
 //
 // All of it is bound by memory: q is read and written once (a thread holds eight channels and their partners half a
 // rotation further, sixteen bytes each), keys and values are read once and written in the order attention reads them.
-// The rotation is computed in 64 bits: its products are exact there (8 by 24 bits), so a rotated value is the exact one
-// rounded once, whatever the angle, and a value on the border of two codes falls on the right side.  The 64-bit units
-// keep up with the memory here (a dozen 64-bit operations per 16 bytes).
+// The rotation is computed in 64 bits, where its products are exact (8 by 24 bits), and rounded to 32 bits and then to bf16:
+// whatever the angle, a rotated value is off by half a step of bf16 and 2^-24 of itself.  Measured, 4 prompts of 1001 to 4097
+// tokens into 4 bits, 16 heads over 2 of 64: 15.5 us, of which the rotation takes 2.8 (12.7 without a table; a copy moves
+// the 51 MB in 10.4); vector units busy 36 % of the time, 28 % without.  7 prompts of 333 to 2100 in bf16, 32 heads over 8 of
+// 128: 37 us for 213 MB.
 #include "paged.h"
 
 #include <numeric>

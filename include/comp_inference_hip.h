@@ -589,21 +589,23 @@ uint32_t ci_debug_wait_limit(uint32_t looks);
  *
  *   ci_kv_cache_bytes    bytes of d_data; 0 for a shape that cannot be (head_dim 64 or 128; page_size a power of two
  *                        from 32 to 4096; kv_heads up to 1024)
- *   ci_paged_kv_append   stores k and v of the new tokens.  With d_rotary (fp32 [rotary_rows, rotary_dim]: cosines, then
- *                        sines, of each position's rotary_dim / 2 angles) keys and, if given, queries are turned by
- *                        their position's angles first: channels d and d + rotary_dim / 2 form a pair, channels from
- *                        rotary_dim on stay.  The rotation is exact up to its one rounding to bf16.  q and q_out (both
- *                        or neither; q_out is q itself or shares no memory with q, k and v) hold q_heads heads.
+ *   ci_paged_kv_append   stores k and v of the new tokens.  With d_rotary (fp32 [rotary_rows, rotary_dim]: cosines,
+ *                        then sines, of each position's rotary_dim / 2 angles) keys and, if given, queries are turned
+ *                        by their position's angles first: channels d and d + rotary_dim / 2 form a pair, channels
+ *                        from rotary_dim on stay.  The rotation is computed in 64 bits and rounded to 32 bits, then
+ *                        to bf16.  q and q_out (both or neither; q_out is q itself or shares no memory with q, k and
+ *                        v) hold q_heads heads.
  *   ci_paged_kv_read     the stored keys and values of the last tokens of every sequence as rows
- *   ci_paged_attention   out = softmax over the visible keys of scale * q k^T, times v: key j is visible to the query at
- *                        position p when j <= p and (window == 0, or p - j < window, or j < sinks).  Query head h reads
- *                        kv head h / (q_heads / kv_heads).  A row that sees no key gets zeros, one
- *                        whose scores are all -inf is NaN.  d_lse (or NULL): fp32
- *                        [rows, q_heads], row stride lse_stride: natural logarithm of the sum of exp(scores), -inf for
- *                        a row without keys.  With a window, pages that hold no key a new token sees need not be named
- *                        (any entry will do).  out shares no memory with q.  max_query_len / max_seq_len: the caller's bounds on the lengths (0: not
- *                        known); they choose kernels, the results do not rest on them.  The workspace is scratch of
- *                        this call: ci_paged_attention_workspace_bytes says how much, for the same arguments.
+ *   ci_paged_attention   out = softmax over the visible keys of scale * q k^T, times v: key j is visible to the query
+ *                        at position p when j <= p and (window == 0, or p - j < window, or j < sinks).  Query head h
+ *                        reads kv head h / (q_heads / kv_heads).  A row that sees no key gets zeros, one whose scores
+ *                        are all -inf is NaN.  d_lse (or NULL): fp32 [rows, q_heads], row stride lse_stride: natural
+ *                        logarithm of the sum of exp(scores), -inf for a row without keys or finite scores.  With a
+ *                        window, pages that hold no key a new token sees need not be named (any entry will do).  out
+ *                        shares no memory with q.  max_query_len / max_seq_len: the caller's bounds on the lengths
+ *                        (0: not known); they choose kernels, the results do not rest on them.  The workspace is
+ *                        scratch of this call: ci_paged_attention_workspace_bytes says how much, for the same
+ *                        arguments.
  * All are enqueued and not waited for, allocate nothing and may be captured.
  * ------------------------------------------------------------------------------------- */
 #define CI_KV_BF16 0u
