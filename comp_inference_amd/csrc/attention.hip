@@ -22,9 +22,11 @@
 //                         1.0 GB: 187 us, 5.4 TB/s; of 48 ragged chats in 4 bits, 0.86 GB: 181 us, 4.7 TB/s.
 //   attend_rows_kernel    for many rows (prompts): bound by the matrix and vector units.  Eight wavefronts of 32 rows share
 //                         the keys and values of a step of 64 tokens through the LDS, in two groups that take turns at the
-//                         matrix unit.  Measured, the same heads: a prompt of 8192 tokens 553 us, 0.99 PFLOP/s (a large
-//                         library product reaches 1.20); the last 1500 tokens each of two sequences of up to 16384 in
-//                         4 bits 930 us, 0.63 PFLOP/s, where the vector unit has the steps and middles to apply as well.
+//                         matrix unit.  Measured, the same heads: a prompt of 8192 tokens 545 us, 1.01 PFLOP/s (a large
+//                         library product reaches 1.20), vector unit busy 42 % and matrix unit 46 % of the time; the last
+//                         1500 tokens each of two sequences of up to 16384 in 4 bits 926 us, 0.63 PFLOP/s, 48 and 26 %:
+//                         the vector unit has the steps and middles to apply as well; ragged prompts under a window of
+//                         1000, 12 heads of 64, 111 us, 48 and 23 %.
 #include "paged.h"
 
 namespace ci {
