@@ -233,11 +233,12 @@ def paged_attention(q, cache: PagedKVCache, block_table, seq_lens, query_start=N
                     scale=None, max_query_len: int = 0, max_seq_len: int = 0, out=None, return_lse: bool = False):
     """softmax(scale * q k^T) v over the visible keys of every query's sequence; q [T, heads, head_dim] in bf16, heads a
     multiple of the cache's kv heads.  The query at position p sees key j when j <= p and, with a `window` > 0, p - j <
-    window or j < `sinks`.  A row that sees nothing (a sequence of length 0) gets zeros, one whose scores are all -inf is NaN; rows behind the last sequence are
-    not written.  With a window, pages that hold no key a new token sees need not be named in `block_table` (any entry
-    will do).  `out` shares no memory with q.  `scale`: 1 / sqrt(head_dim) if not given; positive.  `max_query_len`, `max_seq_len`: what the caller
-    knows about the longest sequence (0: nothing); they choose kernels, the results do not rest on them.  `return_lse`:
-    also fp32 [T, heads], the natural logarithm of the sum of exp(scores).  Scores, sums and the output are held in 32
+    window or j < `sinks`.  A row that sees nothing (a sequence of length 0) gets zeros, one whose scores are all -inf is
+    NaN; rows behind the last sequence are not written.  With a window, pages that hold no key a new token sees need not be
+    named in `block_table` (any entry will do).  `out` shares no memory with q.  `scale`: 1 / sqrt(head_dim) if not given;
+    positive.  `max_query_len`, `max_seq_len`: what the caller knows about the longest sequence (0: nothing); they choose
+    kernels, the results do not rest on them.  `return_lse`: also fp32 [T, heads], the natural logarithm of the sum of
+    exp(scores).  Scores, sums and the output are held in 32
     bits; the weights are rounded to bf16 for the product with v.  No gradients: a q that requires one is refused."""
     _lib.require_device(cache.data)
     _no_gradient(q)

@@ -54,7 +54,7 @@ def test_infinities_and_nan_reach_the_rows_that_see_them(kind, dim, lens, news, 
             mass = mass + R.attention(f.q[at:at + n], k, (R.codes(y) * step).double(), l - n, dim ** -0.5, window, sinks)[0]
         bound = R.attention_bound(want, mass, worst, dim)
         seen = R.visible(l - n + torch.arange(n), l, window, sinks).double()
-        kinds = [(seen @ m.double().reshape(l, -1)).reshape(n, kv_heads, 1, dim).expand(n, kv_heads, heads // kv_heads, dim).reshape(n, heads, dim) > 0
+        kinds = [(seen @ m.double().reshape(l, -1)).reshape(n, kv_heads, dim).repeat_interleave(heads // kv_heads, 1) > 0
                  for m in (x == inf, x == -inf, x.isnan())]
         none = kinds[2] | (kinds[0] & kinds[1])
         y, part = got[at:at + n], lse[at:at + n]
@@ -70,6 +70,37 @@ def test_infinities_and_nan_reach_the_rows_that_see_them(kind, dim, lens, news, 
     assert ci.device_status() == 0
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,news,heads,kv_heads,bounds", CALLS)
+def test_an_infinity_without_weight_is_no_number(dim, lens, news, heads, kv_heads, bounds):
+    """A key whose score is minus infinity weighs nothing, and nothing times an infinity is no number: rows that see it are NaN
+    where its value is infinite, and only there; a key with a weight and an infinity leaves infinities."""
+    ci = _ci()
+    f = Filled(lens, news, heads, kv_heads, dim, "bf16", page=32, seed=23)
+    q = f.q.clone()
+    q[..., 5] = q[..., 5].abs() + 0.5
+    k, v, at = [x.clone() for x in f.k], [x.clone() for x in f.v], 0
+    where = [l - n + n // 2 for l, n in zip(lens, news)]
+    for b, t in enumerate(where):
+        k[b][t, :, 5] = -math.inf
+        v[b][t, :, 8] = math.inf
+        v[b][t, :, 9] = -math.inf
+        v[b][max(t - 1, 0), :, 10] = math.inf
+    whole = torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32).to(DEV)
+    ci.paged_kv_append(f.cache, torch.cat(k).to(DEV), torch.cat(v).to(DEV), f.table, f.seq, whole)
+    got = ci.paged_attention(q.to(DEV), *f.args(), **bounds).cpu()
+    for l, n, t in zip(lens, news, where):
+        p = torch.arange(l - n, l)
+        y = got[at:at + n]
+        assert y[p >= t][..., 8:10].isnan().all() and (y[p >= t - 1][..., 10] == math.inf).all()
+        rest = y.clone()
+        rest[p >= t, :, 8:10] = 0
+        rest[p >= t - 1, :, 10] = 0
+        assert torch.isfinite(rest).all()
+        at += n
+    assert ci.device_status() == 0
+
+
 def _microseconds(call, times=5):
     call()
     begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -82,7 +113,8 @@ def _microseconds(call, times=5):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "int4"])
-@pytest.mark.parametrize("lens,news,heads,kv_heads,least", [([1500], [1500], 16, 8, 30.0), ([20000], [1], 32, 8, 5.0), ([20000], [6], 32, 8, 5.0)])
+@pytest.mark.parametrize("lens,news,heads,kv_heads,least", [([1500], [1500], 16, 8, 30.0), ([20000], [1], 32, 8, 5.0),
+                                                            ([20000], [6], 32, 8, 5.0)])
 def test_a_nan_at_the_first_token_costs_little_time(kind, lens, news, heads, kv_heads, least):
     """Every row sees it, so every row is NaN in that channel, and is computed a second time at a lower rate: three to five
     times the call for a prompt, at most twice for few rows (whose other wavefronts see numbers alone).  Rows done one by one

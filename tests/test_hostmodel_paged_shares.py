@@ -39,9 +39,12 @@ def _joins(log):
     return log.count("attend_rows_join_kernel")
 
 
+MOST = "not (shares and (mixed or (ragged and 128))) and not (see_them and rows and 128)"  # (the longest ones; minutes)
+
+
 def test_the_newer_gpu_tests_on_the_host_model(tmp_path):
-    log = _run(FILES, tmp_path / "launches", least=90)
-    assert _joins(log) >= 70, _joins(log)
+    log = _run(FILES, tmp_path / "launches", pick=MOST, least=80)
+    assert _joins(log) >= 50, _joins(log)
 
 
 PART = "(cut_into_shares and parts) or (see_them and few) or (alone and few_in_shares and 64) or (only and few_several)"
