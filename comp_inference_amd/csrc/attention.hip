@@ -958,7 +958,7 @@ __device__ __forceinline__ TileList tiles_in(const AttendArgs &a, const SeqInfo 
     const int32_t first = s.len - s.n;
     const int32_t x = max(first + (int32_t)token_of(a, kTileRows - 1), 0);
     const int32_t y = max(first + (int32_t)token_of(a, l.tiles * kTileRows - 1), 0);
-    l.pair = (uint32_t)(x + y + 1) / 64 + 2;
+    l.pair = ((uint32_t)x + (uint32_t)y + 1) / 64 + 2;  // (positions up to 2^30 and a tile behind: no room for a sign)
     if (a.window) {  // a tile's steps: the sinks', and those from its first row's window to its last row
         const uint32_t tokens = token_of(a, kTileRows + a.group - 2) + 1;
         l.pair = min(l.pair, 2 * (((uint32_t)a.sinks + kStep - 1) / kStep + ((uint32_t)a.window + tokens) / kStep + 2));
